@@ -397,6 +397,75 @@ int32_t qb_unpatchify(const void* X, const void* W, const void* bias, void* out,
 int32_t qb_patch_gather(const void* latent, void* tokens_out, int32_t C, int32_t H, int32_t Wd, int32_t ph, int32_t pw, void* stream);
 int32_t qb_patch_scatter(const void* tokens_in, void* latent_out, int32_t C, int32_t H, int32_t Wd, int32_t ph, int32_t pw, void* stream);
 
+/* ------------------------------------------------------------------ block-scaled e4m3
+ * Extensions (the reference's e4m3 has no scales): one f32 scale per 128 values of the contraction, for activations per row
+ * (1 x 128 groups), for weights per 128 rows (128 x 128 tiles), the form in which 8-bit checkpoints carry their weights.
+ *
+ *   scale = max(max |x| / 448, 2^-126), 1 for a block of zeros; pow2: rounded up to a power of two
+ *   q     = e4m3(x * (1 / scale))                the quotient, the reciprocal and the product rounded to nearest in f32
+ *
+ * NaN counts for nothing in the maximum and stays NaN; in a block with an infinity the infinities come out as NaN.
+ * Layouts, with kb = ceil(cols / 128): tile_rows 1: scale_out [kb, rows] (the scales of one group of many rows lie together, as
+ * qb_gemm_blocks reads them); tile_rows 128: scale_out [batch, ceil(rows / 128), kb], every matrix of the batch tiled by itself.
+ * row_index (tile_rows 1; may be NULL): out row i and its scales come from row row_index[i] of X; an index outside [0, src_rows)
+ * leaves them as they are (the gather of the experts' rows; s32 [rows]).  cols a multiple of 16. */
+typedef struct {
+  int32_t batch, rows, cols; /* of out; batch 1 with tile_rows 1 */
+  int32_t src_rows;          /* rows of X with tile_rows 1 (== rows without row_index) */
+  int32_t src_dtype;         /* QB_BF16 or QB_F32 */
+  int32_t tile_rows;         /* 1 or 128 */
+  int32_t pow2;
+} qb_quant_blocks_params;
+int32_t qb_quantize_e4m3_blocks(const void* X, const int32_t* row_index, void* out, float* scale_out, const qb_quant_blocks_params* p, void* stream);
+
+/* C[m, n] = epilogue(sum over blocks b of 128 along K of (a_scale[b, m] * b_scale[n / 128, b]) * (A[m, block b] . B[n, block b]))
+ * A [M, K], B [N, K] e4m3, a_scale [ceil(K / 128), M], b_scale [ceil(N / 128), ceil(K / 128)] f32; the sums in f32.  Epilogue as
+ * qb_gemm: -> + bias[n] -> SiLU -> * gate[m / (M / G), n] + residual[m, n] -> cast.  An e4m3 C is narrowed with scales of its own,
+ * c_scale [ceil(N / 128), M] as by qb_quantize_e4m3_blocks from the f32 results: the A operand of a following product.  Else
+ * c_scale is NULL.  K a multiple of 16, N of 8; matrices 16-byte aligned.  Needs no workspace. */
+typedef struct {
+  int32_t M, N, K;
+  int32_t c_dtype;     /* QB_BF16, QB_F32 or QB_E4M3 */
+  int32_t activation;  /* 0 none, 1 SiLU */
+  int32_t gate_groups; /* as qb_gemm_params */
+  int32_t pow2;        /* e4m3 C: scales that are powers of two */
+  int32_t b_constant;  /* as bit 1 of qb_gemm_params.reserved; covers b_scale too */
+  int32_t tile_n;      /* 0 = choose; 64 or 128 */
+  int32_t split_k;     /* 0 = choose; 1, 2, 4 or 8 K slices (more than one: tiles of 64 columns) */
+} qb_gemm_blocks_params;
+int32_t qb_gemm_blocks(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const void* bias, const void* gate,
+                       const void* residual, const qb_gemm_blocks_params* p, void* stream);
+/* The same grouped by expert, as qb_gemm_grouped: tile i (128 rows) of A is multiplied with rows [e N, e N + N) of B, e =
+ * tile_expert[i], and only its first tile_rows[i] rows are written (C and c_scale); tiles with e outside [0, n_experts) are skipped.
+ * B [n_experts * N, K], b_scale [n_experts, ceil(N / 128), ceil(K / 128)], a_scale [ceil(K / 128), M]; plain or SiLU epilogue. */
+int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const int32_t* tile_expert,
+                               const int32_t* tile_rows, int32_t n_experts, const qb_gemm_blocks_params* p, void* stream);
+
+/* ------------------------------------------------------------------ routing by scores
+ * An extension beside qb_moe_route_slots (the reference's "correct" routing).  Per token, over logits l [M, E]:
+ *   s = softmax(l) or sigmoid(l);  c = s + bias (bias f32 [E], may be NULL: it takes part in the choice only)
+ *   the topk_groups of the n_groups groups of E / n_groups neighbouring experts whose best group_top values of c have the largest sum
+ *   experts[m, :] = the top_k experts by c inside them, in order of decreasing c; equal values: the lower group or expert first
+ *   weights[m, j] = s of that expert / (the sum of the chosen ones', with renormalize) * factor
+ * Choices are made on c as the formula has it, not on a rounding to f32.  A logit of -inf has score 0, and a sum of 0 gives weights
+ * 0 (a row without any finite logit).  NaN is chosen last and reaches the weights.  E <= 512, n_groups <= 32, top_k <= 32.
+ * The slot tables (all or none of the five pointers), for n = qb_moe_scored_slots(M, E, top_k) slots, a multiple of 128 that any
+ * routing fits: slot_token, slot_weight, tile_expert, token_slot as in qb_moe_route_slots, and tile_rows [n / 128], the slots of each
+ * tile that hold a token (0 past the last used tile).  Workspace (may be NULL up to 64 tokens or without tables): the first 64 KiB
+ * are not touched, so that the workspace of qb_gemm can be lent; calls that share one must not overlap. */
+typedef struct {
+  int32_t M, E, top_k;
+  int32_t logits_dtype; /* QB_BF16 or QB_F32 */
+  int32_t scoring;      /* 0 softmax, 1 sigmoid */
+  int32_t n_groups, topk_groups, group_top; /* group_top 1 or 2; n_groups 1: no groups */
+  int32_t renormalize;
+  float factor;
+} qb_route_params;
+size_t qb_moe_scored_slots(int32_t M, int32_t E, int32_t top_k);
+size_t qb_moe_route_scored_workspace_bytes(const qb_route_params* p);
+int32_t qb_moe_route_scored(const void* logits, const float* bias, int32_t* experts, float* weights, int32_t* slot_token, float* slot_weight, int32_t* tile_expert,
+                            int32_t* tile_rows, int32_t* token_slot, const qb_route_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ one session over several GPUs
  * The reference is single-GPU (ref: src/quark/models/waypoint_15.py:318, :333: B = 1, one device); nothing below has a
  * counterpart there.  When a block is sharded by KV-head group, out-proj and fc2 are row-parallel and their partial

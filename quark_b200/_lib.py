@@ -82,6 +82,18 @@ class TpParams(C.Structure):
     ]  # fmt: skip
 
 
+class QuantBlocksParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("batch", "rows", "cols", "src_rows", "src_dtype", "tile_rows", "pow2")]
+
+
+class GemmBlocksParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("M", "N", "K", "c_dtype", "activation", "gate_groups", "pow2", "b_constant", "tile_n", "split_k")]
+
+
+class RouteParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("M", "E", "top_k", "logits_dtype", "scoring", "n_groups", "topk_groups", "group_top", "renormalize")] + [("factor", C.c_float)]
+
+
 _P, _I, _Z, _F, _U = C.c_void_p, C.c_int32, C.c_size_t, C.c_float, C.c_uint32
 
 # name -> (restype, argtypes); every symbol include/quark_b200.h declares
@@ -158,6 +170,12 @@ SIGNATURES = {
     "qb_gemm_grouped_workspace_bytes": (_Z, [C.POINTER(GemmParams)]),
     "qb_gemm_grouped": (_I, [_P, _P, _P, _P, _I, C.POINTER(GemmParams), _P, _Z, _P]),
     "qb_moe_reduce": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
+    "qb_quantize_e4m3_blocks": (_I, [_P, _P, _P, _P, C.POINTER(QuantBlocksParams), _P]),
+    "qb_gemm_blocks": (_I, [_P] * 9 + [C.POINTER(GemmBlocksParams), _P]),
+    "qb_gemm_grouped_blocks": (_I, [_P] * 8 + [_I, C.POINTER(GemmBlocksParams), _P]),
+    "qb_moe_scored_slots": (_Z, [_I, _I, _I]),
+    "qb_moe_route_scored_workspace_bytes": (_Z, [C.POINTER(RouteParams)]),
+    "qb_moe_route_scored": (_I, [_P] * 9 + [C.POINTER(RouteParams), _P, _Z, _P]),
     "qb_tp_arena_bytes": (_Z, [_I, _I]),
     "qb_tp_arena_offsets": (_I, [_I, _I, C.POINTER(_Z)]),
     "qb_tp_reduce": (_I, [_P, _P, _P, _P, C.POINTER(TpParams), _P]),
@@ -198,7 +216,8 @@ def load():
 
 # The entry points that csrc/fastcall.c calls by address.
 FASTCALL = ("qb_gemm", "qb_gemm_workspace_bytes", "qb_ada_rmsnorm", "qb_ada_rmsnorm_chained", "qb_rmsnorm", "qb_head_rmsnorm", "qb_ada_gate_residual", "qb_silu", "qb_add",
-            "qb_euler_step", "qb_quantize_e4m3", "qb_dequantize_e4m3", "qb_kv_cache_update", "qb_kv_cache_update_kv", "qb_owl_attn_scratch_bytes", "qb_owl_attn")  # fmt: skip
+            "qb_euler_step", "qb_quantize_e4m3", "qb_dequantize_e4m3", "qb_kv_cache_update", "qb_kv_cache_update_kv", "qb_owl_attn_scratch_bytes", "qb_owl_attn",
+            "qb_quantize_e4m3_blocks", "qb_gemm_blocks", "qb_gemm_grouped_blocks", "qb_moe_scored_slots", "qb_moe_route_scored_workspace_bytes", "qb_moe_route_scored")  # fmt: skip
 
 
 class _NoFastcall:

@@ -133,6 +133,16 @@ __device__ __forceinline__ float silu_fast(float x) {
   return fmaf(h, t, h);
 }
 
+// The scale of a block of values that becomes e4m3, from its largest magnitude (see blocks.cu).
+__device__ __forceinline__ float block_scale(float top, bool pow2) {
+  if (top == 0.f) return 1.f;
+  if (!pow2 || isinf(top)) return fmaxf(__fdiv_rn(top, 448.f), 1.17549435e-38f);
+  // the smallest 2^j with top <= 448 * 2^j = 1.75 * 2^(j + 8)
+  const int bits = __float_as_int(top), e = (bits >> 23) - 127;
+  const int j = (bits & 0x7fffff) <= 0x600000 ? e - 8 : e - 7;
+  return __int_as_float((max(j, -126) + 127) << 23);
+}
+
 // 32-byte global stores (one full sector per thread); the address must be 32-byte aligned.
 __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),

@@ -32,6 +32,14 @@ typedef size_t (*attn_ws_fn)(const qb_attn_params*);
 typedef int32_t (*attn_fn)(const void*, const void*, const void*, const int32_t*, const int32_t*, const int32_t*, void*, void*, const float*, const qb_attn_params*, void*,
                            size_t, void*);
 
+typedef int32_t (*quant_blocks_fn)(const void*, const int32_t*, void*, float*, const qb_quant_blocks_params*, void*);
+typedef int32_t (*gemm_blocks_fn)(const void*, const void*, const float*, const float*, void*, float*, const void*, const void*, const void*, const qb_gemm_blocks_params*, void*);
+typedef int32_t (*grouped_blocks_fn)(const void*, const void*, const float*, const float*, void*, float*, const int32_t*, const int32_t*, int32_t, const qb_gemm_blocks_params*,
+                                     void*);
+typedef size_t (*slots_fn)(int32_t, int32_t, int32_t);
+typedef size_t (*route_ws_fn)(const qb_route_params*);
+typedef int32_t (*route_fn)(const void*, const float*, int32_t*, float*, int32_t*, float*, int32_t*, int32_t*, int32_t*, const qb_route_params*, void*, size_t, void*);
+
 static struct {
   gemm_fn gemm;
   gemm_ws_fn gemm_ws;
@@ -49,6 +57,12 @@ static struct {
   append_kv_fn append_kv;
   attn_ws_fn attn_ws;
   attn_fn attn;
+  quant_blocks_fn quant_blocks;
+  gemm_blocks_fn gemm_blocks;
+  grouped_blocks_fn grouped_blocks;
+  slots_fn scored_slots;
+  route_ws_fn route_ws;
+  route_fn route;
 } g_lib;
 
 typedef struct {
@@ -342,6 +356,127 @@ static PyObject* fast_owl_attn(PyObject* self, PyObject* const* a, Py_ssize_t n)
   RUN(g_lib.attn(Q.ptr, Kc.ptr, Vc.ptr, seg.ptr, nseg.ptr, ft.ptr, out.ptr, oq.ptr, rope.ptr, &p, need > 0 ? ws.ptr : NULL, need > 0 ? (size_t)ws.nbytes : 0, st));
 }
 
+static int flag_of(PyObject* o, int32_t* v) {
+  *v = o == Py_True;
+  return o == Py_True || o == Py_False;
+}
+static long long blocks128(long long n) { return (n + 127) / 128; }
+
+/* (X, row_index, out, scale_out, tile_rows, pow2, stream) */
+static PyObject* fast_quantize_blocks(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  Tensor X, idx, out, sc;
+  long long tile;
+  qb_quant_blocks_params p;
+  void* st;
+  if (n != 7 || g_lib.quant_blocks == NULL || !tensor(a[0], &X) || !tensor_or_none(a[1], &idx) || !tensor(a[2], &out) || !tensor(a[3], &sc) || !as_ll(a[4], &tile) ||
+      !flag_of(a[5], &p.pow2) || !stream_of(a[6], &st))
+    Py_RETURN_NONE;
+  const Py_ssize_t nd = PyTuple_GET_SIZE(X.shape);
+  const long long cols = dim(&X, -1);
+  if (nd < 2 || (X.dtype != QB_BF16 && X.dtype != QB_F32) || out.dtype != QB_E4M3 || sc.dtype != QB_F32 || !SMALL(cols) || cols % 16 != 0 || X.numel <= 0) Py_RETURN_NONE;
+  long long batch = 1, rows, src;
+  if (tile == 128) {
+    if (nd > 3 || idx.ptr != NULL) Py_RETURN_NONE;
+    batch = nd == 3 ? dim(&X, 0) : 1;
+    src = rows = dim(&X, -2);
+  } else {
+    if (tile != 1 || (idx.ptr != NULL && idx.dtype != QB_S32)) Py_RETURN_NONE;
+    src = X.numel / cols;
+    rows = idx.ptr != NULL ? idx.numel : src;
+  }
+  if (!SMALL(batch) || !SMALL(rows) || !SMALL(src) || out.numel != batch * rows * cols || sc.numel != blocks128(cols) * (tile == 1 ? rows : batch * blocks128(rows))) Py_RETURN_NONE;
+  p.batch = (int32_t)batch; p.rows = (int32_t)rows; p.cols = (int32_t)cols; p.src_rows = (int32_t)src; p.src_dtype = X.dtype; p.tile_rows = (int32_t)tile;
+  RUN(g_lib.quant_blocks(X.ptr, (const int32_t*)idx.ptr, out.ptr, (float*)sc.ptr, &p, st));
+}
+
+/* out and its scales against [M, N]: 1 where they go together */
+static int blocks_output(PyObject* want, const Tensor* out, const Tensor* sc, long long M, long long N) {
+  if (out->dtype < 0 || out->dtype == QB_S32 || out->numel != M * N || (want != Py_None && dtype_code(want) != out->dtype)) return 0;
+  return out->dtype == QB_E4M3 ? sc->ptr != NULL && sc->dtype == QB_F32 && sc->numel == blocks128(N) * M : sc->ptr == NULL;
+}
+
+/* (A, B, a_scale, b_scale, out_dtype, activation, bias, gate, residual, gate_groups, out, scale_out, pow2, b_constant, tile_n, split_k, stream) */
+static PyObject* fast_gemm_blocks(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  Tensor A, B, sa, sb, bias, gate, res, out, sc;
+  long long groups, tile, split;
+  qb_gemm_blocks_params p;
+  void* st;
+  if (n != 17 || g_lib.gemm_blocks == NULL || !tensor(a[0], &A) || !tensor(a[1], &B) || !tensor(a[2], &sa) || !tensor(a[3], &sb) || !tensor_or_none(a[6], &bias) ||
+      !tensor_or_none(a[7], &gate) || !tensor_or_none(a[8], &res) || !as_ll(a[9], &groups) || !tensor(a[10], &out) || !tensor_or_none(a[11], &sc) || !flag_of(a[12], &p.pow2) ||
+      !flag_of(a[13], &p.b_constant) || !as_ll(a[14], &tile) || !as_ll(a[15], &split) || !stream_of(a[16], &st))
+    Py_RETURN_NONE;
+  const int act = activation_of(a[5]);
+  const long long K = dim(&A, -1), N = dim(&B, 0);
+  if (act < 0 || PyTuple_GET_SIZE(A.shape) < 2 || PyTuple_GET_SIZE(B.shape) != 2 || A.dtype != QB_E4M3 || B.dtype != QB_E4M3 || sa.dtype != QB_F32 || sb.dtype != QB_F32 ||
+      !SMALL(K) || !SMALL(N) || dim(&B, 1) != K || !SMALL(groups) || !SMALL(A.numel / K) || tile < 0 || tile > 256 || split < 0 || split > 16)
+    Py_RETURN_NONE;
+  const long long M = A.numel / K, kb = blocks128(K);
+  if (sa.numel != kb * M || sb.numel != blocks128(N) * kb || !blocks_output(a[4], &out, &sc, M, N) || (bias.ptr != NULL && (bias.dtype != QB_BF16 || bias.numel != N)) ||
+      (gate.ptr == NULL) != (res.ptr == NULL))
+    Py_RETURN_NONE;
+  if (gate.ptr != NULL && (gate.dtype != QB_BF16 || res.dtype != QB_BF16 || gate.numel != groups * N || res.numel != M * N || M % groups != 0)) Py_RETURN_NONE;
+  p.M = (int32_t)M; p.N = (int32_t)N; p.K = (int32_t)K; p.c_dtype = out.dtype; p.activation = act; p.gate_groups = (int32_t)groups;
+  p.tile_n = (int32_t)tile; p.split_k = (int32_t)split;
+  RUN(g_lib.gemm_blocks(A.ptr, B.ptr, (const float*)sa.ptr, (const float*)sb.ptr, out.ptr, (float*)sc.ptr, bias.ptr, gate.ptr, res.ptr, &p, st));
+}
+
+/* (A, B, a_scale, b_scale, tile_expert, tile_rows, n_experts, out_dtype, activation, out, scale_out, pow2, b_constant, tile_n, stream) */
+static PyObject* fast_gemm_grouped_blocks(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  Tensor A, B, sa, sb, te, tr, out, sc;
+  long long E, tile;
+  qb_gemm_blocks_params p;
+  void* st;
+  if (n != 15 || g_lib.grouped_blocks == NULL || !tensor(a[0], &A) || !tensor(a[1], &B) || !tensor(a[2], &sa) || !tensor(a[3], &sb) || !tensor(a[4], &te) ||
+      !tensor(a[5], &tr) || !as_ll(a[6], &E) || !tensor(a[9], &out) || !tensor_or_none(a[10], &sc) || !flag_of(a[11], &p.pow2) || !flag_of(a[12], &p.b_constant) ||
+      !as_ll(a[13], &tile) || !stream_of(a[14], &st))
+    Py_RETURN_NONE;
+  const int act = activation_of(a[8]);
+  const long long K = dim(&A, -1);
+  if (act < 0 || PyTuple_GET_SIZE(A.shape) < 2 || PyTuple_GET_SIZE(B.shape) < 2 || A.dtype != QB_E4M3 || B.dtype != QB_E4M3 || sa.dtype != QB_F32 || sb.dtype != QB_F32 ||
+      te.dtype != QB_S32 || tr.dtype != QB_S32 || !SMALL(K) || dim(&B, -1) != K || !SMALL(E) || !SMALL(A.numel / K) || !SMALL(B.numel / K) || B.numel / K % E != 0 || tile < 0 ||
+      tile > 256)
+    Py_RETURN_NONE;
+  const long long M = A.numel / K, N = B.numel / K / E, kb = blocks128(K);
+  if (M % 128 != 0 || N == 0 || sa.numel != kb * M || sb.numel != E * blocks128(N) * kb || te.numel != M / 128 || tr.numel != M / 128 || !blocks_output(a[7], &out, &sc, M, N))
+    Py_RETURN_NONE;
+  p.M = (int32_t)M; p.N = (int32_t)N; p.K = (int32_t)K; p.c_dtype = out.dtype; p.activation = act; p.gate_groups = 1;
+  p.tile_n = (int32_t)tile; p.split_k = 0;
+  RUN(g_lib.grouped_blocks(A.ptr, B.ptr, (const float*)sa.ptr, (const float*)sb.ptr, out.ptr, (float*)sc.ptr, (const int32_t*)te.ptr, (const int32_t*)tr.ptr, (int32_t)E, &p, st));
+}
+
+/* (logits, bias, top_k, scoring, n_groups, topk_groups, group_top, renormalize, factor, tables, out, workspace, stream) */
+static PyObject* fast_route_scored(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  Tensor l, bias, ws, o[7];
+  long long k, groups, kept, top;
+  int32_t tables;
+  qb_route_params p;
+  void* st;
+  if (n != 13 || g_lib.route == NULL || !tensor(a[0], &l) || !tensor_or_none(a[1], &bias) || !as_ll(a[2], &k) || !as_ll(a[4], &groups) || !as_ll(a[5], &kept) ||
+      !as_ll(a[6], &top) || !flag_of(a[7], &p.renormalize) || !as_float(a[8], &p.factor) || !flag_of(a[9], &tables) || (!PyList_CheckExact(a[10]) && !PyTuple_Check(a[10])) ||
+      !tensor_or_none(a[11], &ws) || !stream_of(a[12], &st) || !PyUnicode_Check(a[3]))
+    Py_RETURN_NONE;
+  const int sigmoid = PyUnicode_CompareWithASCIIString(a[3], "sigmoid") == 0;
+  const long long M = dim(&l, 0), E = dim(&l, 1);
+  if ((!sigmoid && PyUnicode_CompareWithASCIIString(a[3], "softmax") != 0) || (l.dtype != QB_BF16 && l.dtype != QB_F32) || PyTuple_GET_SIZE(l.shape) != 2 || !SMALL(M) ||
+      E <= 0 || E > 512 || k <= 0 || k > 32 || k > E || groups < 1 || groups > 32 || E % groups != 0 || kept < 1 || kept > groups || kept * (E / groups) < k || top < 1 || top > 2 ||
+      (groups > 1 && E / groups < top) || (bias.ptr != NULL && (bias.dtype != QB_F32 || bias.numel != E)))
+    Py_RETURN_NONE;
+  const long long slots = (long long)g_lib.scored_slots((int32_t)M, (int32_t)E, (int32_t)k);
+  const long long numel[7] = {M * k, M * k, slots, slots, slots / 128, slots / 128, M * k};
+  static const int dtypes[7] = {QB_S32, QB_F32, QB_S32, QB_F32, QB_S32, QB_S32, QB_S32};
+  const Py_ssize_t want = tables ? 7 : 2;
+  PyObject* const seq = a[10];
+  if (slots == 0 || PySequence_Fast_GET_SIZE(seq) != want) Py_RETURN_NONE;
+  memset(o, 0, sizeof(o));
+  for (Py_ssize_t i = 0; i < want; ++i)
+    if (!tensor(PySequence_Fast_GET_ITEM(seq, i), &o[i]) || o[i].numel != numel[i] || o[i].dtype != dtypes[i]) Py_RETURN_NONE;
+  p.M = (int32_t)M; p.E = (int32_t)E; p.top_k = (int32_t)k; p.logits_dtype = l.dtype; p.scoring = sigmoid;
+  p.n_groups = (int32_t)groups; p.topk_groups = (int32_t)kept; p.group_top = (int32_t)top;
+  if (tables && g_lib.route_ws(&p) > (size_t)ws.nbytes) Py_RETURN_NONE;
+  RUN(g_lib.route(l.ptr, (const float*)bias.ptr, (int32_t*)o[0].ptr, (float*)o[1].ptr, (int32_t*)o[2].ptr, (float*)o[3].ptr, (int32_t*)o[4].ptr, (int32_t*)o[5].ptr,
+                  (int32_t*)o[6].ptr, &p, ws.ptr, (size_t)ws.nbytes, st));
+}
+
 /* (tensor class, {entry point: address}) */
 static PyObject* fast_bind(PyObject* self, PyObject* args) {
   PyObject *cls, *table;
@@ -356,11 +491,12 @@ static PyObject* fast_bind(PyObject* self, PyObject* args) {
     }
     *at[i] = ((PyMemberDescrObject*)d)->d_member->offset;
   }
-  static const char* const names[16] = {"qb_gemm", "qb_gemm_workspace_bytes", "qb_ada_rmsnorm", "qb_ada_rmsnorm_chained", "qb_rmsnorm", "qb_head_rmsnorm", "qb_ada_gate_residual",
+  static const char* const names[22] = {"qb_gemm", "qb_gemm_workspace_bytes", "qb_ada_rmsnorm", "qb_ada_rmsnorm_chained", "qb_rmsnorm", "qb_head_rmsnorm", "qb_ada_gate_residual",
                                         "qb_silu", "qb_add", "qb_euler_step", "qb_quantize_e4m3", "qb_dequantize_e4m3", "qb_kv_cache_update",
-                                        "qb_kv_cache_update_kv", "qb_owl_attn_scratch_bytes", "qb_owl_attn"};
+                                        "qb_kv_cache_update_kv", "qb_owl_attn_scratch_bytes", "qb_owl_attn", "qb_quantize_e4m3_blocks", "qb_gemm_blocks",
+                                        "qb_gemm_grouped_blocks", "qb_moe_scored_slots", "qb_moe_route_scored_workspace_bytes", "qb_moe_route_scored"};
   void** const fn = (void**)&g_lib;
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 22; ++i) {
     PyObject* v = PyDict_GetItemString(table, names[i]);
     if (v == NULL) {
       PyErr_Format(PyExc_KeyError, "bind: %s", names[i]);
@@ -377,7 +513,8 @@ static PyObject* fast_bind(PyObject* self, PyObject* args) {
 
 #define F(name) {#name, (PyCFunction)(void (*)(void))fast_##name, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {{"bind", fast_bind, METH_VARARGS, NULL}, F(gemm), F(ada_rmsnorm), F(rmsnorm), F(head_rmsnorm), F(gate_residual), F(silu),
-                                F(add), F(euler_step), F(quantize), F(dequantize), F(kv_cache_update), F(owl_attn), {NULL, NULL, 0, NULL}};
+                                F(add), F(euler_step), F(quantize), F(dequantize), F(kv_cache_update), F(owl_attn), F(quantize_blocks),
+                                F(gemm_blocks), F(gemm_grouped_blocks), F(route_scored), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__fastcall(void) {

@@ -1,0 +1,515 @@
+// Matrix products of block-scaled e4m3 operands: C[m, n] = epilogue(sum over blocks b of 128 along K of
+// a_scale[b, m] * b_scale[n / 128, b] * (A[m, block b] . B[n, block b])), dense and grouped by expert.
+//
+// The scales change along the contraction, so the tensor cores can sum one block only: four MMAs (32 of K each) fill one of four TMEM
+// buffers of BN columns, and while they fill the next ones, the eight warps of the epilogue read it and add it, scaled, to
+// sums in registers (f32; two warps share a TMEM lane quarter, each thread has half a row).  A block of K is one stage of the operand ring: 128 rows
+// x 128 bytes of A, BN x 128 of B.  When the last block is in, the sums go back to TMEM, from where the plain epilogue takes
+// them 16 columns at a time.
+//
+// Warp 0 TMA, warp 1 MMA, warps 2-9 sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
+#include <atomic>
+
+#include "gemm_common.cuh"
+
+namespace qb {
+
+constexpr int kAccBuffers = 4;
+
+struct BlockArgs {
+  GemmArgs g;
+  const float* a_scale;  // [kb_total][M]
+  const float* b_scale;  // [N / 128 (of every expert)][kb_total]
+  float* c_scale;        // [N / 128][M], e4m3 C
+  const int* tile_rows;  // grouped: slots of a tile that hold a token
+  int pow2, n_experts;
+  int small_rows;  // rows of A in the box of the second map (grouped)
+};
+
+template <int BN>
+struct BlockSmem {
+  static constexpr int kStageBytes = (kBM + BN) * kRowBytes;
+  static constexpr int kSliceBytes = BN == 64 ? kBM * BN * 4 : 0;  // partial sums that the cluster's other K slices push
+  static constexpr int kStages = BN == 64 ? 7 : 6;
+  static constexpr int kSliceOffset = kStages * kStageBytes;
+  static constexpr int kBarOffset = kSliceOffset + kSliceBytes;
+  static constexpr int kColOffset = kBarOffset + 256;  // per-column scale (unused), bias, gate
+  static constexpr int kTopOffset = kColOffset + 3 * BN * 4;
+  static constexpr int kTotal = kTopOffset + 2 * kBM * 4 + 1024;  // + alignment slack
+  static_assert((2 * kStages + 2 * kAccBuffers) * 8 + 32 <= 256 && kTotal <= 227 * 1024, "shared memory of one CTA");
+};
+
+// d += a * b on two f32 at once
+__device__ __forceinline__ void fma2(float2& d, float ax, float ay, float2 b) {
+  asm("{\n\t.reg .b64 p, q, r;\n\t"
+      "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tmov.b64 r, {%4, %5};\n\t"
+      "fma.rn.f32x2 p, q, r, p;\n\t"
+      "mov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(d.x), "+f"(d.y)
+      : "f"(ax), "f"(ay), "f"(b.x), "f"(b.y));
+}
+
+template <int BN, bool GROUPED>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_small, const __grid_constant__ CUtensorMap tmB, const BlockArgs args) {
+  using L = BlockSmem<BN>;
+  constexpr int kStages = L::kStages;
+  constexpr uint32_t kTmemCols = kAccBuffers * BN;
+  constexpr uint32_t kIdesc = umma_idesc(0, 0, kBM, BN);
+  constexpr int kHalf = BN / 2;  // columns of a thread
+  const GemmArgs& g = args.g;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* acc_full = empty_bar + kStages;       // [buffer] a block's products are complete
+  uint64_t* acc_empty = acc_full + kAccBuffers;   // [buffer] the eight warps have read them
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccBuffers);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* drain_flag = abort_flag + 1;  // never set: lets the drain waits below run their own limit
+  volatile int* lost_flag = abort_flag + 2;   // set by a CTA of the cluster whose slice is missing
+  float* col = reinterpret_cast<float*>(smem + L::kColOffset);
+  float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // [half][row]: largest magnitude of half a row
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * kBM, split = blockIdx.z;
+  const int kb0 = split * g.kb_per_split, n_iter = min(kb0 + g.kb_per_split, g.kb_total) - kb0;
+  const bool clustered = BN == 64 && g.cluster != 0;
+  int expert = 0, rows = min(g.M - m0, kBM);
+  if (GROUPED) {
+    grid_dep_wait();  // the tables are written by the routing kernel
+    grid_dep_launch();
+    expert = after_wait(g.tile_expert)[blockIdx.y];
+    if (expert < 0 || expert >= args.n_experts) return;  // a padding tile
+    rows = min(max(after_wait(args.tile_rows)[blockIdx.y], 0), kBM);
+    if (rows == 0) return;
+  }
+  const bool small = GROUPED && rows <= args.small_rows;
+  const int a_rows = small ? args.small_rows : g.a_rows;
+  const uint32_t stage_tx = a_rows * kRowBytes + BN * kRowBytes;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(small ? &tmA_small : &tmA);
+    tma_prefetch_desc(&tmB);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < kAccBuffers; ++b) {
+      mbar_init(smem_u32(&acc_full[b]), 1);
+      mbar_init(smem_u32(&acc_empty[b]), 8);
+    }
+    *abort_flag = 0;
+    *drain_flag = 0;
+    *lost_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  if (clustered) cluster_sync();  // every CTA of the cluster is there before anyone pushes to it
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if (!GROUPED) grid_dep_launch();
+
+  if (warp == 0) {
+    // ---------------- TMA producer
+    if (elect_one()) {
+      const CUtensorMap* a_map = small ? &tmA_small : &tmA;
+      const int b_row0 = expert * g.N + n0;
+      // constant weights do not depend on the kernels before this one: their first tiles are on the way while those finish
+      const int ahead = !GROUPED && g.b_const ? min(kStages, n_iter) : 0;
+      for (int it = 0; it < ahead; ++it) {
+        const uint32_t fb = smem_u32(&full_bar[it]);
+        mbar_arrive_expect_tx(fb, stage_tx);
+        tma_load_2d(smem_u32(smem + it * L::kStageBytes + kBM * kRowBytes), &tmB, fb, (kb0 + it) * 128, b_row0);
+      }
+      if (!GROUPED) grid_dep_wait();
+      for (int it = 0; it < ahead; ++it) tma_load_2d(smem_u32(smem + it * L::kStageBytes), a_map, smem_u32(&full_bar[it]), (kb0 + it) * 128, m0);
+      int issued = ahead;
+      for (int it = ahead; it < n_iter; ++it) {
+        const int s = it % kStages;
+        const uint32_t ph = (it / kStages) & 1;
+        if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        const uint32_t fb = smem_u32(&full_bar[s]), st = smem_u32(smem + s * L::kStageBytes);
+        mbar_arrive_expect_tx(fb, stage_tx);
+        tma_load_2d(st + kBM * kRowBytes, &tmB, fb, (kb0 + it) * 128, b_row0);
+        tma_load_2d(st, a_map, fb, (kb0 + it) * 128, m0);
+        issued = it + 1;
+      }
+      if (*abort_flag) {
+        // Giving up: let the copies already in flight land before this CTA's memory goes away.
+        for (int it = max(0, issued - kStages); it < issued; ++it)
+          mbar_wait(smem_u32(&full_bar[it % kStages]), (it / kStages) & 1, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+      } else {
+        // Tail: see the last stage releases land before the CTA can exit.
+        for (int it = max(0, n_iter - kStages); it < n_iter; ++it)
+          if (!mbar_wait(smem_u32(&empty_bar[it % kStages]), (it / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer: one block of K into one buffer
+    if (elect_one()) {
+      bool ok = true;
+      for (int it = 0; it < n_iter && ok; ++it) {
+        const int s = it % kStages, buf = it % kAccBuffers;
+        ok = mbar_wait(smem_u32(&full_bar[s]), (it / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+        if (ok && it >= kAccBuffers)
+          ok = mbar_wait(smem_u32(&acc_empty[buf]), (it / kAccBuffers - 1) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a_addr = smem_u32(smem + s * L::kStageBytes);
+        const uint64_t a_desc = umma_desc_k_sw128(a_addr), b_desc = umma_desc_k_sw128(a_addr + kBM * kRowBytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_f8(tmem_base + buf * BN, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&empty_bar[s]));
+        if (it == n_iter - 1 && late(blockIdx.x == gridDim.x - 1 && blockIdx.z == gridDim.z - 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        umma_commit(smem_u32(&acc_full[buf]));  // (not reached: the other warps give up as well)
+      }
+    }
+  } else {
+    // ---------------- sums and epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31
+    const int lane_grp = warp & 3, half = (warp - 2) >> 2, et = threadIdx.x - 64;
+    const int row = lane_grp * 32 + lane, m = m0 + row;
+    const bool live = row < rows, busy = lane_grp * 32 < rows;  // this thread's row, any row of this warp
+    if (!GROUPED) grid_dep_wait();
+    const int m_last = m0 + rows - 1;
+    const bool one_gate = g.gate == nullptr || m0 / g.rows_per_gate == m_last / g.rows_per_gate;
+    const int slice_rows = kBM / (clustered ? g.splits : 1), slice_row0 = clustered ? split * slice_rows : 0;  // rows this CTA finishes
+    const float* as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + m;
+    const float* bs = after_wait(args.b_scale) + static_cast<size_t>(expert * ((g.N + 127) / 128) + n0 / 128) * g.kb_total + kb0;
+    float sc[4];  // scales of the next four blocks
+    auto scale_of = [&](int it) { return it < n_iter && live ? as[static_cast<size_t>(it) * g.M] * bs[it] : 0.f; };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sc[j] = scale_of(j);
+    // the tile's per-column vectors, and the residuals of the 8-column groups that this thread finishes for the cluster
+    for (int j = et; j < BN; j += 256) {
+      const int n = n0 + j;
+      const bool in = n < g.N;
+      col[BN + j] = (in && g.bias) ? bf16_bits_to_f32(g.bias[n]) : 0.f;
+      col[2 * BN + j] = (in && g.gate) ? bf16_bits_to_f32(g.gate[static_cast<size_t>(m0 / g.rows_per_gate) * g.N + n]) : 0.f;
+    }
+    uint4 pre[BN / 32][2];
+    if (clustered && one_gate && g.gate != nullptr) {
+#pragma unroll
+      for (int k = 0; k < BN / 32; ++k) {
+        const int r = et / (BN / 8) + 256 / (BN / 8) * k, mm = m0 + slice_row0 + r, n = n0 + et % (BN / 8) * 8;
+        pre[k][0] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < slice_rows && mm < g.M && n < g.N) pre[k][0] = *reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(mm) * g.N + n);
+      }
+    }
+    asm volatile("bar.sync 2, 256;" ::: "memory");
+
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_grp * 32) << 16) + half * kHalf;
+    float2 acc[kHalf / 2];
+#pragma unroll
+    for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int base = 0; base < n_iter && ok; base += kAccBuffers) {
+#pragma unroll
+      for (int j = 0; j < kAccBuffers; ++j) {
+        const int it = base + j;
+        if (it >= n_iter) break;
+        const float s = sc[j];
+        sc[j] = scale_of(it + 4);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&acc_full[j]), (it / kAccBuffers) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t t[kHalf / 32][32];
+        if (busy) {
+#pragma unroll
+          for (int c = 0; c < kHalf / 32; ++c) tmem_ld32(taddr + j * BN + c * 32, t[c]);
+          tmem_wait_ld_into(t[0]);
+#pragma unroll
+          for (int c = 1; c < kHalf / 32; ++c) tmem_loaded(t[c]);
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j]));
+        if (busy) {
+          const float2 s2 = make_float2(s, s);
+#pragma unroll
+          for (int c = 0; c < kHalf / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], __uint_as_float(t[c][2 * i]), __uint_as_float(t[c][2 * i + 1]), s2);
+        }
+      }
+    }
+    const bool precise = g.c_dtype != QB_BF16;
+    if (clustered) {
+      if constexpr (BN == 64) {
+        ok = all_of_epilogue(ok);
+        if (ok) {
+          const uint32_t dst = map_to_cta(smem_u32(smem + L::kSliceOffset), row / slice_rows);
+#pragma unroll
+          for (int v = 0; v < kHalf / 4; ++v)
+            st_dsmem_v4(dst + 16 * slice_unit<BN>(split, half * (kHalf / 4) + v, row % slice_rows, slice_rows), __float_as_uint(acc[2 * v].x), __float_as_uint(acc[2 * v].y),
+                        __float_as_uint(acc[2 * v + 1].x), __float_as_uint(acc[2 * v + 1].y));
+        } else if (threadIdx.x == 64) {
+          tell_lost<1>(lost_flag, 0, g.splits);
+        }
+        cluster_sync();  // every slice's share of this CTA's rows has arrived after this barrier (warps 0 and 1 join it below)
+        if (ok && *lost_flag == 0) {
+          const float4* parts = reinterpret_cast<const float4*>(smem + L::kSliceOffset);
+          if (precise) finish_slices<BN, true>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
+          else finish_slices<BN, false>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
+        }
+      }
+    } else {
+      const bool narrow = args.c_scale != nullptr;
+      if (narrow) ok = all_of_epilogue(ok);  // its two halves of a row meet at a barrier
+      if (ok && busy) {
+        // every MMA of the CTA is done (this warp has waited for each block), and a warp reads back what it wrote itself
+#pragma unroll
+        for (int c = 0; c < kHalf / 32; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            w[2 * i] = __float_as_uint(acc[c * 16 + i].x);
+            w[2 * i + 1] = __float_as_uint(acc[c * 16 + i].y);
+          }
+          tmem_st32(taddr + c * 32, w);
+        }
+        tmem_wait_st();
+        const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.C) & 31u) == 0;
+        uint8_t* c_row = live ? row_of_c(g, m) : nullptr;
+        const uint4* res_row = reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(m) * g.N + n0);
+        const int c0 = half * kHalf;
+        uint4 next[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};  // residual of the next turn
+        auto fetch = [&](int c) {
+          if (g.gate != nullptr && c < c0 + kHalf && live && n0 + c < g.N) {
+            next[0] = res_row[c / 8];
+            if (n0 + c + 8 < g.N) next[1] = res_row[c / 8 + 1];
+          }
+        };
+        fetch(c0);
+        float top = 0.f;
+#pragma unroll 1
+        for (int c = c0; c < c0 + kHalf; c += 16) {
+          if (n0 + c >= g.N) break;
+          uint4 res[2] = {next[0], next[1]};
+          uint32_t r[16];
+          tmem_ld16(taddr + c - c0, r);
+          fetch(c + 16);
+          tmem_wait_ld_into(r);
+          if (!narrow) {
+            if (!live) continue;
+            if (precise) epilogue16<BN, true>(g, r, m, n0 + c, col + c, res, one_gate, c_row, wide, true);
+            else epilogue16<BN, false>(g, r, m, n0 + c, col + c, res, one_gate, c_row, wide, true);
+          } else {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+            if (live) epilogue16_values<BN, true>(g, v, m, n0 + c, col + c, res, one_gate);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (j < 8 || n0 + c + 8 < g.N) top = fmaxf(top, fabsf(v[j]));
+              r[j] = __float_as_uint(v[j]);
+            }
+            tmem_st16(taddr + c - c0, r);
+          }
+        }
+        if (narrow) {
+          tmem_wait_st();
+          tops[half * kBM + row] = top;
+        }
+      }
+      if constexpr (BN == 128) {
+        if (narrow && ok) {
+          asm volatile("bar.sync 2, 256;" ::: "memory");
+          if (busy) {
+            const float s = block_scale(fmaxf(tops[row], tops[kBM + row]), args.pow2 != 0), inv = __frcp_rn(s);
+            if (live && half == 0) args.c_scale[static_cast<size_t>(n0 / 128) * g.M + m] = s;
+            uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
+            const bool wide = g.N % 16 == 0;
+#pragma unroll 1
+            for (int c = half * kHalf; c < (half + 1) * kHalf; c += 16) {
+              const int n = n0 + c;
+              if (n >= g.N) break;
+              uint32_t r[16], w[4];
+              tmem_ld16(taddr + c - half * kHalf, r);
+              tmem_wait_ld_into(r);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = pack_e4m3x4(__fmul_rn(__uint_as_float(r[4 * j]), inv), __fmul_rn(__uint_as_float(r[4 * j + 1]), inv), __fmul_rn(__uint_as_float(r[4 * j + 2]), inv),
+                                   __fmul_rn(__uint_as_float(r[4 * j + 3]), inv));
+              if (!live) continue;
+              if (wide) {
+                *reinterpret_cast<uint4*>(c_row + n) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
+                *reinterpret_cast<uint2*>(c_row + n) = make_uint2(w[0], w[1]);
+                if (n + 8 < g.N) *reinterpret_cast<uint2*>(c_row + n + 8) = make_uint2(w[2], w[3]);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  if (clustered && warp < 2) {
+    __syncwarp();
+    cluster_sync();  // the barrier after which the epilogue warps read what was pushed to them
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct BlockPlan {
+  int bn, splits, kb_total, kb_per_split;
+};
+
+// Width of the tiles and number of K slices.
+static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
+  const int kb_total = (p.K + 127) / 128, sms = num_sms();
+  BlockPlan best{128, 1, kb_total, kb_total};
+  if (p.c_dtype == QB_E4M3) return best;  // a group of 128 results is one tile's
+  double best_cost = 1e30;
+  for (int bn = 64; bn <= 128; bn += 64) {
+    if (p.tile_n != 0 && p.tile_n != bn) continue;
+    if (bn == 128 && p.tile_n == 0 && p.N <= 64) continue;
+    for (int s = 1; s <= (bn == 64 ? 8 : 1); s *= 2) {
+      if (p.split_k != 0 && p.split_k != s) continue;
+      const int kbps = (kb_total + s - 1) / s;
+      if ((kb_total + kbps - 1) / kbps != s || (s > 1 && p.split_k == 0 && kbps < 4)) continue;
+      const long tiles = static_cast<long>(row_tiles) * ((p.N + bn - 1) / bn);
+      const long slots = s == 4 ? 33 : s == 8 ? 15 : sms / s;  // clusters that run at once
+      const long rounds = (tiles + slots - 1) / slots;
+      const double body = kbps * (bn == 64 ? 150.0 : 200.0);
+      double cost = 3500.0 + body + (rounds - 1) * (body + 2500.0);
+      if (s > 1) cost += 300.0 + 12.0 * tiles * s;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = BlockPlan{bn, s, kb_total, kbps};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BN, bool GROUPED>
+static int32_t launch_blocks(const CUtensorMap& tmA, const CUtensorMap& tmA_small, const CUtensorMap& tmB, const BlockArgs& a, dim3 grid, cudaStream_t st) {
+  using L = BlockSmem<BN>;
+  static std::atomic<unsigned long long> configured{0};  // one bit per device
+  int dev = 0;
+  QB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || (configured.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+    QB_CUDA_OK(cudaFuncSetAttribute(gemm_blocks_kernel<BN, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+    if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = L::kTotal;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (g_dependent_launch) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (a.g.cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = static_cast<unsigned>(a.g.splits);
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_blocks_kernel<BN, GROUPED>, tmA, tmA_small, tmB, a);
+  ++g_launch_count;
+  if (e != cudaSuccess) return fail(QB_ERR_LAUNCH, "gemm kernel (block scales, %d columns, %d slices): %s", BN, a.g.splits, cudaGetErrorString(e));
+  return QB_OK;
+}
+
+static int32_t validate_blocks(const qb_gemm_blocks_params* p) {
+  QB_REQUIRE(p != nullptr, QB_ERR_INVALID_ARG, "gemm_blocks: params are NULL");
+  QB_REQUIRE(p->M > 0 && p->N > 0 && p->K > 0, QB_ERR_INVALID_ARG, "gemm_blocks: M, N, K must be positive (got %d, %d, %d)", p->M, p->N, p->K);
+  QB_REQUIRE(p->c_dtype == QB_BF16 || p->c_dtype == QB_F32 || p->c_dtype == QB_E4M3, QB_ERR_INVALID_ARG, "gemm_blocks: c_dtype %d", p->c_dtype);
+  QB_REQUIRE(p->K % 16 == 0, QB_ERR_ALIGN, "gemm_blocks: K = %d must be a multiple of 16", p->K);
+  QB_REQUIRE(p->N % 8 == 0, QB_ERR_ALIGN, "gemm_blocks: N = %d must be a multiple of 8", p->N);
+  QB_REQUIRE(p->activation == 0 || p->activation == 1, QB_ERR_INVALID_ARG, "gemm_blocks: activation %d", p->activation);
+  QB_REQUIRE(p->tile_n == 0 || p->tile_n == 64 || p->tile_n == 128, QB_ERR_INVALID_ARG, "gemm_blocks: tile_n %d", p->tile_n);
+  QB_REQUIRE(p->split_k >= 0 && p->split_k <= 8, QB_ERR_INVALID_ARG, "gemm_blocks: split_k %d", p->split_k);
+  QB_REQUIRE(p->M <= 65535 * kBM, QB_ERR_INVALID_ARG, "gemm_blocks: %d rows", p->M);
+  return QB_OK;
+}
+
+static int32_t blocks_run(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const void* bias, const void* gate,
+                          const void* residual, const int* tile_expert, const int* tile_rows, int n_experts, const qb_gemm_blocks_params* p, cudaStream_t st) {
+  int32_t rc = validate_blocks(p);
+  if (rc != QB_OK) return rc;
+  QB_REQUIRE(A && B && C && a_scale && b_scale, QB_ERR_INVALID_ARG, "gemm_blocks: A, B, C and the scales must not be NULL");
+  QB_REQUIRE((gate == nullptr) == (residual == nullptr), QB_ERR_INVALID_ARG, "gemm_blocks: gate and residual come together");
+  QB_REQUIRE((c_scale != nullptr) == (p->c_dtype == QB_E4M3), QB_ERR_INVALID_ARG, "gemm_blocks: an e4m3 C has scales, another has none");
+  QB_REQUIRE(aligned16(A) && aligned16(B) && aligned16(C) && aligned16(bias) && aligned16(gate) && aligned16(residual), QB_ERR_ALIGN,
+             "gemm_blocks: every matrix must be 16-byte aligned");
+  QB_REQUIRE(((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale) | reinterpret_cast<uintptr_t>(c_scale)) & 3u) == 0, QB_ERR_ALIGN,
+             "gemm_blocks: scales must be 4-byte aligned");
+  unsigned int* status = status_word();
+  QB_REQUIRE(status != nullptr, QB_ERR_CUDA, "gemm_blocks: device status word unavailable");
+  const bool grouped = tile_expert != nullptr;
+  BlockArgs a{};
+  GemmArgs& g = a.g;
+  g.rows_per_gate = p->M;
+  if (gate != nullptr) {
+    QB_REQUIRE(p->gate_groups >= 1 && p->M % p->gate_groups == 0, QB_ERR_INVALID_ARG, "gemm_blocks: gate_groups %d does not divide M = %d", p->gate_groups, p->M);
+    g.rows_per_gate = p->M / p->gate_groups;
+  }
+  const int row_tiles = (p->M + kBM - 1) / kBM;
+  const BlockPlan pl = plan_blocks(*p, row_tiles);
+  g.M = p->M; g.N = p->N; g.K = p->K;
+  g.a_rows = p->M < kBM ? (p->M + 7) / 8 * 8 : kBM;
+  g.kb_total = pl.kb_total; g.kb_per_split = pl.kb_per_split; g.splits = pl.splits; g.cluster = pl.splits > 1;
+  g.b_const = p->b_constant != 0;
+  g.c_dtype = p->c_dtype; g.activation = p->activation;
+  g.bias = static_cast<const uint16_t*>(bias);
+  g.gate = static_cast<const uint16_t*>(gate);
+  g.residual = static_cast<const uint16_t*>(residual);
+  g.C = C;
+  g.status = status;
+  g.tile_expert = tile_expert;
+  a.a_scale = a_scale; a.b_scale = b_scale; a.c_scale = c_scale; a.tile_rows = tile_rows; a.pow2 = p->pow2 != 0; a.n_experts = n_experts;
+  a.small_rows = grouped ? 32 : 0;
+  CUtensorMap tmA, tmA_small, tmB;
+  rc = make_tmap_2d_sw(&tmA, A, 1, p->M, p->K, g.a_rows, 128, 128);
+  if (rc != QB_OK) return rc;
+  tmA_small = tmA;
+  if (grouped) {
+    rc = make_tmap_2d_sw(&tmA_small, A, 1, p->M, p->K, a.small_rows, 128, 128);
+    if (rc != QB_OK) return rc;
+  }
+  rc = make_tmap_2d_sw(&tmB, B, 1, static_cast<uint64_t>(p->N) * n_experts, p->K, pl.bn, 128, 128);
+  if (rc != QB_OK) return rc;
+  const dim3 grid((p->N + pl.bn - 1) / pl.bn, row_tiles, pl.splits);
+  if (grouped) return pl.bn == 128 ? launch_blocks<128, true>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, true>(tmA, tmA_small, tmB, a, grid, st);
+  return pl.bn == 128 ? launch_blocks<128, false>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, false>(tmA, tmA_small, tmB, a, grid, st);
+}
+
+}  // namespace qb
+
+using namespace qb;
+
+extern "C" int32_t qb_gemm_blocks(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const void* bias, const void* gate,
+                                  const void* residual, const qb_gemm_blocks_params* p, void* stream) {
+  return blocks_run(A, B, a_scale, b_scale, C, c_scale, bias, gate, residual, nullptr, nullptr, 1, p, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const int32_t* tile_expert,
+                                          const int32_t* tile_rows, int32_t n_experts, const qb_gemm_blocks_params* p, void* stream) {
+  QB_REQUIRE(p != nullptr && tile_expert != nullptr && tile_rows != nullptr, QB_ERR_INVALID_ARG, "gemm_grouped_blocks: params or tile tables are NULL");
+  QB_REQUIRE(p->M > 0 && p->M % kBM == 0, QB_ERR_UNSUPPORTED, "gemm_grouped_blocks: M = %d must be a multiple of 128", p->M);
+  QB_REQUIRE(n_experts >= 1 && static_cast<long long>(n_experts) * p->N < (1ll << 31), QB_ERR_INVALID_ARG, "gemm_grouped_blocks: %d experts", n_experts);
+  qb_gemm_blocks_params q = *p;
+  q.split_k = 1;  // a padding tile leaves before any K slice could wait for it
+  return blocks_run(A, B, a_scale, b_scale, C, c_scale, nullptr, nullptr, nullptr, tile_expert, tile_rows, n_experts, &q, static_cast<cudaStream_t>(stream));
+}

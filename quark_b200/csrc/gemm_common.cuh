@@ -66,7 +66,14 @@ struct GemmArgs {
   int tiles_m, n_tiles, group_m, stages, scratch;
 };
 
+// SiLU of a GEMM's epilogue.  kPrecise: where the approximation's 2^-11 would be seen in the result (f32, or e4m3 with scales of its own).
+template <bool kPrecise>
+__device__ __forceinline__ float epilogue_silu(float x) {
+  return kPrecise ? __fdividef(x, 1.f + __expf(-x)) : silu_fast(x);
+}
+
 // Applies the epilogue to 8 consecutive columns of one row and stores them.
+template <bool kPrecise = false>
 __device__ __forceinline__ void epilogue_store8(const GemmArgs& g, float (&v)[8], int m, int n) {
   if (g.a_scale != nullptr || g.w_scale != nullptr) {
     const float sa = g.a_scale ? *g.a_scale : 1.0f;
@@ -84,7 +91,7 @@ __device__ __forceinline__ void epilogue_store8(const GemmArgs& g, float (&v)[8]
   }
   if (g.activation == 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = silu_fast(v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = epilogue_silu<kPrecise>(v[j]);
   }
   if (g.gate != nullptr) {
     const size_t grow = static_cast<size_t>(m / g.rows_per_gate) * g.N;
@@ -120,7 +127,7 @@ __device__ __forceinline__ void epilogue_store8(const GemmArgs& g, float (&v)[8]
 
 // The same on values that were fetched ahead: `col` points at this column's scale, with the bias BN and the gate 2 BN words
 // further, and `rs` is the residual.
-template <int BN>
+template <int BN, bool kPrecise = false>
 __device__ __forceinline__ void epilogue_store8_staged(const GemmArgs& g, float (&v)[8], int m, int n, const float* col, const uint4& rs) {
   if (g.a_scale != nullptr || g.w_scale != nullptr) {
 #pragma unroll
@@ -132,7 +139,7 @@ __device__ __forceinline__ void epilogue_store8_staged(const GemmArgs& g, float 
   }
   if (g.activation == 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = silu_fast(v[j]);
+    for (int j = 0; j < 8; ++j) v[j] = epilogue_silu<kPrecise>(v[j]);
   }
   if (g.gate != nullptr) {
     const uint32_t rw[4] = {rs.x, rs.y, rs.z, rs.w};
@@ -204,7 +211,7 @@ __device__ __forceinline__ bool all_of_epilogue(bool ok) {
 
 // After the cluster barrier: this CTA's rows of the tile, 8 columns at a time per thread (neighbouring threads take neighbouring
 // groups of a row, so that whole lines are read and written), summed in slice order.  pre[k][0]: the residuals.
-template <int BN>
+template <int BN, bool kPrecise = false>
 __device__ __forceinline__ void finish_slices(const GemmArgs& g, const float4* parts, const float* col, int m0, int n0, int row0, int rows, bool one_gate,
                                               const uint4 (&pre)[BN / 32][2]) {
   const int et = threadIdx.x - 64, c8 = et % (BN / 8);
@@ -219,8 +226,8 @@ __device__ __forceinline__ void finish_slices(const GemmArgs& g, const float4* p
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
       v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
-    if (one_gate) epilogue_store8_staged<BN>(g, v, m, n, col + c8 * 8, pre[k][0]);
-    else epilogue_store8(g, v, m, n);
+    if (one_gate) epilogue_store8_staged<BN, kPrecise>(g, v, m, n, col + c8 * 8, pre[k][0]);
+    else epilogue_store8<kPrecise>(g, v, m, n);
   }
 }
 
@@ -234,15 +241,10 @@ __device__ __forceinline__ uint8_t* row_of_c(const GemmArgs& g, int m) {
   return static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N * es;
 }
 
-// The plain epilogue on 16 columns of one row: r the accumulator, `col` at the first column's scale (bias BN, gate 2 BN words
-// further), `res` the residual.  Kept small and called in a loop: unrolled over the half row, with every branch in it, the
-// epilogue's instructions cost more to fetch (0.5 us a launch) than they took to run.
-template <int BN>
-__device__ __forceinline__ void epilogue16(const GemmArgs& g, const uint32_t (&r)[16], int m, int n, const float* col, const uint4* res, bool one_gate,
-                                           uint8_t* c_row, bool wide, bool store) {
-  float v[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+// What the plain epilogue makes of 16 columns of one row: v the accumulator, `col` at the first column's scale (bias BN, gate 2 BN
+// words further), `res` the residual.
+template <int BN, bool kPrecise = false>
+__device__ __forceinline__ void epilogue16_values(const GemmArgs& g, float (&v)[16], int m, int n, const float* col, const uint4* res, bool one_gate) {
   if (g.a_scale != nullptr || g.w_scale != nullptr) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] *= col[j];
@@ -253,7 +255,7 @@ __device__ __forceinline__ void epilogue16(const GemmArgs& g, const uint32_t (&r
   }
   if (g.activation == 1) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = silu_fast(v[j]);
+    for (int j = 0; j < 16; ++j) v[j] = epilogue_silu<kPrecise>(v[j]);
   }
   const bool second = n + 8 < g.N;
   if (g.gate != nullptr) {
@@ -275,6 +277,18 @@ __device__ __forceinline__ void epilogue16(const GemmArgs& g, const uint32_t (&r
       }
     }
   }
+}
+
+// The plain epilogue on 16 columns of one row: r the accumulator, the others as above.  Kept small and called in a loop: unrolled
+// over the half row, with every branch in it, the epilogue's instructions cost more to fetch (0.5 us a launch) than they took to run.
+template <int BN, bool kPrecise = false>
+__device__ __forceinline__ void epilogue16(const GemmArgs& g, const uint32_t (&r)[16], int m, int n, const float* col, const uint4* res, bool one_gate,
+                                           uint8_t* c_row, bool wide, bool store) {
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+  epilogue16_values<BN, kPrecise>(g, v, m, n, col, res, one_gate);
+  const bool second = n + 8 < g.N;
   if (!store) {  // (the values still have to be worked out: see the caller)
 #pragma unroll
     for (int j = 0; j < 16; ++j) asm volatile("" ::"f"(v[j]));

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 from collections import OrderedDict
+from typing import NamedTuple
 
 import numpy as np
 
@@ -22,6 +23,7 @@ from ..runtime.tensor import QuarkTensor
 __all__ = [
     "gemm", "owl_attn", "kv_cache_update", "quantize_e4m3", "ada_rmsnorm", "head_rmsnorm", "value_residual_packed",
     "ada_gate_residual", "silu", "euler_step", "patchify", "unpatchify", "increment", "rope_table", "qkv_post", "quantize_e4m3_rows",
+    "quantize_e4m3_blocks", "gemm_blocks", "gemm_grouped_blocks", "moe_route_scored", "moe_scored_slots", "Routing",
 ]  # fmt: skip
 
 
@@ -356,6 +358,174 @@ def dequantize_e4m3(X, *, out=None):
         raise ValueError("qf.dequantize_e4m3: out must be a bf16 tensor of the same size")
     _lib.check(_lib.load().qb_dequantize_e4m3(_p(X), _p(out), X.numel, _s()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# block-scaled e4m3 (extensions: the reference's e4m3 has no scales)
+# ---------------------------------------------------------------------------
+
+BLOCK = 128  # values of the contraction under one scale, and rows of a weight
+
+
+def _ceil_div(a: int, b: int) -> int:
+    return -(-a // b)
+
+
+def _matrix(who, name, t, dtype, numel, shape):
+    """``t`` is of ``dtype`` and holds the elements of ``shape``."""
+    if _dt(t) != dtype:
+        raise TypeError(f"{who}: {name} dtype {_dt(t)!r} (expected {dtype})")
+    if t.numel != numel:
+        raise ValueError(f"{who}: {name} is {tuple(t.shape)}, expected {shape}")
+
+
+def quantize_e4m3_blocks(X, *, tile_rows: int = 1, pow2: bool = False, row_index=None, out=None, scale_out=None):
+    """bf16 / f32 ``[rows, cols]`` -> e4m3 with one f32 scale per block of 128 columns: ``scale = max|x| / 448`` (1 for a block of
+    zeros; with ``pow2`` rounded up to a power of two), ``q = e4m3(x * (1 / scale))``.  Returns ``(out, scale_out)``.
+
+    ``tile_rows=1`` (activations): a scale per row and block, ``scale_out [ceil(cols / 128), rows]``.  ``tile_rows=128`` (weights):
+    a scale per 128 x 128 tile, ``[ceil(rows / 128), ceil(cols / 128)]``; ``X`` may then be a batch ``[B, rows, cols]`` of matrices
+    with tiles of their own.  ``row_index`` (s32, ``tile_rows=1``): row ``i`` of the result comes from row ``row_index[i]`` of ``X``,
+    an index outside ``X`` leaves row and scales as they are (the gather of the experts' rows)."""
+    who = "qf.quantize_e4m3_blocks"
+    if out is not None and scale_out is not None:
+        rc = _fast.quantize_blocks(X, row_index, out, scale_out, tile_rows, pow2, _s())
+        if rc is not None:
+            if rc:
+                _lib.check(rc)
+            return out, scale_out
+    dt = _dt(X)
+    if dt not in ("bf16", "f32"):
+        raise TypeError(f"{who}: source dtype {dt!r} is not supported")
+    if tile_rows not in (1, BLOCK):
+        raise ValueError(f"{who}: tile_rows {tile_rows!r} (1 or 128)")
+    cols = int(X.shape[-1]) if X.ndim >= 2 else 0
+    if X.numel == 0 or cols == 0 or cols % 16:
+        raise ValueError(f"{who}: X is {tuple(X.shape)}, expected at least one row and a multiple of 16 columns")
+    kb = _ceil_div(cols, BLOCK)
+    if tile_rows == BLOCK:
+        if row_index is not None:
+            raise ValueError(f"{who}: row_index goes with tile_rows=1")
+        if X.ndim > 3:
+            raise ValueError(f"{who}: X is {tuple(X.shape)}, expected a matrix or a batch of them")
+        batch, rows = (int(X.shape[0]) if X.ndim == 3 else 1), int(X.shape[-2])
+        src, shape = rows, tuple(X.shape)
+        s_shape = ((batch,) if X.ndim == 3 else ()) + (_ceil_div(rows, BLOCK), kb)
+    else:
+        batch, src = 1, X.numel // cols
+        if row_index is not None and _dt(row_index) != "s32":
+            raise TypeError(f"{who}: row_index dtype {_dt(row_index)!r} (expected s32)")
+        rows = src if row_index is None else row_index.numel
+        if rows == 0:
+            raise ValueError(f"{who}: row_index is empty")
+        shape, s_shape = (tuple(X.shape) if row_index is None else (rows, cols)), (kb, rows)
+    if out is None:
+        out = QuarkTensor.empty(*shape, dtype="e4m3")
+    if scale_out is None:
+        scale_out = QuarkTensor.empty(*s_shape, dtype="f32")
+    _matrix(who, "out", out, "e4m3", batch * rows * cols, shape)
+    _matrix(who, "scale_out", scale_out, "f32", int(np.prod(s_shape)), s_shape)
+    p = _lib.QuantBlocksParams(batch, rows, cols, src, _lib.DTYPE_CODE[dt], int(tile_rows), 1 if pow2 else 0)
+    _lib.check(_lib.load().qb_quantize_e4m3_blocks(_p(X), _p(row_index), _p(out), _p(scale_out), C.byref(p), _s()))
+    return out, scale_out
+
+
+def _blocks_outputs(who, M, N, out_dtype, out, scale_out):
+    od = _name(out_dtype)
+    if od is None:
+        od = _dt(out) if out is not None else "e4m3" if scale_out is not None else "bf16"
+    if od not in ("bf16", "f32", "e4m3"):
+        raise TypeError(f"{who}: out dtype {od!r} is not supported")
+    if out is None:
+        out = QuarkTensor.empty(M, N, dtype=od)
+    elif out.numel != M * N or _dt(out) != od:
+        raise ValueError(f"{who}: out is {tuple(out.shape)} {_dt(out)}, expected ({M}, {N}) {od}")
+    if od != "e4m3":
+        if scale_out is not None:
+            raise ValueError(f"{who}: scale_out goes with an e4m3 result")
+    elif scale_out is None:
+        scale_out = QuarkTensor.empty(_ceil_div(N, BLOCK), M, dtype="f32")
+    else:
+        _matrix(who, "scale_out", scale_out, "f32", _ceil_div(N, BLOCK) * M, (_ceil_div(N, BLOCK), M))
+    return od, out, scale_out
+
+
+def gemm_blocks(A, B, a_scale, b_scale, *, out_dtype=None, activation=None, bias=None, gate=None, residual=None, gate_groups=1, out=None, scale_out=None,
+                pow2=False, b_constant=False, tile_n=0, split_k=0):  # fmt: skip
+    """``C = A @ B.T`` of block-scaled e4m3 operands (+ bias, SiLU, ``residual + gate * C`` as ``gemm``): block ``b`` of 128 along K
+    counts ``a_scale[b, m] * b_scale[n // 128, b]`` times.  ``A [M, K]`` and ``a_scale [ceil(K / 128), M]`` as ``quantize_e4m3_blocks``
+    makes them of activations, ``B [N, K]`` and ``b_scale [ceil(N / 128), ceil(K / 128)]`` as it makes them of a weight
+    (``tile_rows=128``); any f32 scales do.
+
+    An e4m3 result (``out_dtype="e4m3"``, or an e4m3 ``out``) is narrowed with scales of its own and returned as ``(out, scale_out)``, the A operand
+    of a following product.  ``b_constant`` as in ``gemm``, for ``B`` and ``b_scale``."""
+    who = "qf.gemm_blocks"
+    if out is not None:
+        rc = _fast.gemm_blocks(A, B, a_scale, b_scale, out_dtype, activation, bias, gate, residual, gate_groups, out, scale_out, pow2, b_constant, tile_n, split_k, _s())
+        if rc is not None:
+            if rc:
+                _lib.check(rc)
+            return out if scale_out is None else (out, scale_out)
+    if A.ndim < 2 or B.ndim != 2:
+        raise ValueError(f"{who}: A must be at least rank-2 and B rank-2, got {A.shape} and {B.shape}")
+    K, N = int(A.shape[-1]), int(B.shape[0])
+    if K == 0 or A.numel == 0 or N == 0 or int(B.shape[1]) != K:
+        raise ValueError(f"{who}: A is {tuple(A.shape)} but B is {tuple(B.shape)} (expected [N, {K}], none of them empty)")
+    M, kb = A.numel // K, _ceil_div(K, BLOCK)
+    _matrix(who, "A", A, "e4m3", M * K, (M, K))
+    _matrix(who, "B", B, "e4m3", N * K, (N, K))
+    _matrix(who, "a_scale", a_scale, "f32", kb * M, (kb, M))
+    _matrix(who, "b_scale", b_scale, "f32", _ceil_div(N, BLOCK) * kb, (_ceil_div(N, BLOCK), kb))
+    if activation not in (None, "silu"):
+        raise ValueError(f"{who}: unsupported activation {activation!r}")
+    if (gate is None) != (residual is None):
+        raise ValueError(f"{who}: gate and residual must be given together")
+    if bias is not None:
+        _matrix(who, "bias", bias, "bf16", N, (N,))
+    if gate is not None:
+        if gate_groups < 1 or M % gate_groups:
+            raise ValueError(f"{who}: gate_groups={gate_groups} does not divide M={M}")
+        _matrix(who, "gate", gate, "bf16", gate_groups * N, (gate_groups, N))
+        _matrix(who, "residual", residual, "bf16", M * N, (M, N))
+    od, out, scale_out = _blocks_outputs(who, M, N, out_dtype, out, scale_out)
+    p = _lib.GemmBlocksParams(M, N, K, _code(od), 1 if activation == "silu" else 0, int(gate_groups), 1 if pow2 else 0, 1 if b_constant else 0, int(tile_n), int(split_k))
+    _lib.check(_lib.load().qb_gemm_blocks(_p(A), _p(B), _p(a_scale), _p(b_scale), _p(out), _p(scale_out), _p(bias), _p(gate), _p(residual), C.byref(p), _s()))
+    return out if scale_out is None else (out, scale_out)
+
+
+def gemm_grouped_blocks(A, B, a_scale, b_scale, tile_expert, tile_rows, *, n_experts: int, out_dtype=None, activation=None, out=None, scale_out=None, pow2=False,
+                        b_constant=False, tile_n=0):  # fmt: skip
+    """``gemm_blocks`` over 128-row tiles of slot-sorted rows, every tile with the weights of its expert (``gemm_grouped``): ``B`` is
+    ``[n_experts * N, K]`` and ``b_scale [n_experts, ceil(N / 128), ceil(K / 128)]`` (``quantize_e4m3_blocks`` of ``[n_experts, N, K]``).
+    The first ``tile_rows[i]`` rows of tile ``i`` are written, the others, and tiles without an expert, are left as they are."""
+    who = "qf.gemm_grouped_blocks"
+    if out is not None:
+        rc = _fast.gemm_grouped_blocks(A, B, a_scale, b_scale, tile_expert, tile_rows, n_experts, out_dtype, activation, out, scale_out, pow2, b_constant, tile_n, _s())
+        if rc is not None:
+            if rc:
+                _lib.check(rc)
+            return out if scale_out is None else (out, scale_out)
+    if A.ndim < 2 or B.ndim < 2:
+        raise ValueError(f"{who}: A and B must be at least rank-2, got {A.shape} and {B.shape}")
+    K = int(A.shape[-1])
+    if K == 0 or A.numel == 0 or B.numel == 0 or int(B.shape[-1]) != K or n_experts < 1 or (B.numel // K) % n_experts:
+        raise ValueError(f"{who}: A is {tuple(A.shape)} but B is {tuple(B.shape)} (expected [{n_experts} * N, {K}], none of them empty)")
+    M, N, kb = A.numel // K, B.numel // K // n_experts, _ceil_div(K, BLOCK)
+    if M % 128:
+        raise ValueError(f"{who}: {M} rows are no whole tiles")
+    _matrix(who, "A", A, "e4m3", M * K, (M, K))
+    _matrix(who, "B", B, "e4m3", n_experts * N * K, (n_experts * N, K))
+    _matrix(who, "a_scale", a_scale, "f32", kb * M, (kb, M))
+    _matrix(who, "b_scale", b_scale, "f32", n_experts * _ceil_div(N, BLOCK) * kb, (n_experts, _ceil_div(N, BLOCK), kb))
+    _matrix(who, "tile_expert", tile_expert, "s32", M // 128, (M // 128,))
+    _matrix(who, "tile_rows", tile_rows, "s32", M // 128, (M // 128,))
+    if activation not in (None, "silu"):
+        raise ValueError(f"{who}: unsupported activation {activation!r}")
+    od, out, scale_out = _blocks_outputs(who, M, N, out_dtype, out, scale_out)
+    p = _lib.GemmBlocksParams(M, N, K, _code(od), 1 if activation == "silu" else 0, 1, 1 if pow2 else 0, 1 if b_constant else 0, int(tile_n), 0)
+    _lib.check(_lib.load().qb_gemm_grouped_blocks(_p(A), _p(B), _p(a_scale), _p(b_scale), _p(out), _p(scale_out), _p(tile_expert), _p(tile_rows), int(n_experts),
+                                                  C.byref(p), _s()))  # fmt: skip
+    return out if scale_out is None else (out, scale_out)
 
 
 # ---------------------------------------------------------------------------
@@ -932,6 +1102,70 @@ def moe_reduce(partials, slot_weight, token_slot, *, out=None):
         raise ValueError(f"qf.moe_reduce: out must be bf16 [{M}, {D}]")
     _lib.check(_lib.load().qb_moe_reduce(_p(partials), _p(slot_weight), _p(token_slot), _p(out), M, D, top_k, _s()))
     return out
+
+
+class Routing(NamedTuple):
+    """What ``moe_route_scored`` returns: every token's experts and weights, and the slot tables of the experts' products (None without)."""
+
+    experts: QuarkTensor
+    weights: QuarkTensor
+    slot_token: QuarkTensor | None
+    slot_weight: QuarkTensor | None
+    tile_expert: QuarkTensor | None
+    tile_rows: QuarkTensor | None
+    token_slot: QuarkTensor | None
+
+
+def moe_scored_slots(M: int, E: int, top_k: int) -> int:
+    """Slots that the tables of ``moe_route_scored`` have: whole 128-row tiles that any routing fits."""
+    return int(_lib.load().qb_moe_scored_slots(int(M), int(E), int(top_k)))
+
+
+def moe_route_scored(logits, bias=None, *, top_k: int, scoring: str = "softmax", n_groups: int = 1, topk_groups: int = 1, group_top: int = 1,
+                     renormalize: bool = True, factor: float = 1.0, tables: bool = True, out=None) -> Routing:  # fmt: skip
+    """Routing by scores, an extension beside the reference's "correct" routing (``moe_route_slots``).
+
+    ``s`` is the softmax or the sigmoid of the logits (bf16 or f32 ``[M, E]``), ``c = s + bias`` (f32 ``[E]``; it takes part in the choice only).  The
+    ``topk_groups`` of the ``n_groups`` groups of neighbouring experts whose best ``group_top`` values of ``c`` have the largest sum are
+    kept, and a token goes to the ``top_k`` experts of largest ``c`` inside them (equal values: the lower group or expert first), with
+    the weights ``s`` (over the chosen ones' sum, with ``renormalize``) times ``factor``.  A logit of ``-inf`` scores 0 (a bias of ``-inf``
+    takes an expert out of the choice while others are left); where the chosen scores sum to 0, the weights are 0.  ``out``: the seven tensors of a ``Routing`` to be written (the first two with ``tables=False``)."""
+    who = "qf.moe_route_scored"
+    if out is not None:
+        rc = _fast.route_scored(logits, bias, top_k, scoring, n_groups, topk_groups, group_top, renormalize, factor, tables, out, _WS, _s())
+        if rc is not None:
+            if rc:
+                _lib.check(rc)
+            return Routing(*out) if tables else Routing(out[0], out[1], None, None, None, None, None)
+    dt = _dt(logits)
+    if dt not in ("bf16", "f32") or logits.ndim != 2:
+        raise TypeError(f"{who}: logits must be a bf16 or f32 [M, E] tensor")
+    if scoring not in ("softmax", "sigmoid"):
+        raise ValueError(f"{who}: scoring {scoring!r} (softmax or sigmoid)")
+    M, E, k = int(logits.shape[0]), int(logits.shape[1]), int(top_k)
+    if bias is not None:
+        _matrix(who, "bias", bias, "f32", E, (E,))
+    lib = _lib.load()
+    p = _lib.RouteParams(M, E, k, _lib.DTYPE_CODE[dt], 1 if scoring == "sigmoid" else 0, int(n_groups), int(topk_groups), int(group_top), 1 if renormalize else 0, float(factor))
+    n = moe_scored_slots(M, E, k)
+    if n == 0 or k > 32 or E > 512:
+        raise ValueError(f"{who}: top_k {k} of {E} experts for {M} tokens (at most 32 of 512)")
+    if not (1 <= n_groups <= 32) or E % n_groups or not (1 <= topk_groups <= n_groups) or topk_groups * (E // n_groups) < k:
+        raise ValueError(f"{who}: {topk_groups} of {n_groups} groups (at most 32) of {E} experts for top_k {k}")
+    if group_top not in (1, 2) or (n_groups > 1 and E // n_groups < group_top):
+        raise ValueError(f"{who}: group_top {group_top} (1 or 2, at most a group's {E // n_groups} experts)")
+    spec = [("experts", "s32", (M, k)), ("weights", "f32", (M, k)), ("slot_token", "s32", (n,)), ("slot_weight", "f32", (n,)), ("tile_expert", "s32", (n // 128,)),
+            ("tile_rows", "s32", (n // 128,)), ("token_slot", "s32", (M, k))][: 7 if tables else 2]  # fmt: skip
+    if out is None:
+        out = [QuarkTensor.empty(*shape, dtype=d) for _, d, shape in spec]
+    elif len(out) != len(spec):
+        raise ValueError(f"{who}: out holds {len(out)} tensors, expected {[name for name, _, _ in spec]}")
+    for t, (name, d, shape) in zip(out, spec):
+        _matrix(who, name, t, d, int(np.prod(shape)), shape)
+    ptrs = [t.data_ptr() for t in out] + [None] * (7 - len(out))
+    ws = _workspace(int(lib.qb_moe_route_scored_workspace_bytes(C.byref(p))) if tables else 0)
+    _lib.check(lib.qb_moe_route_scored(_p(logits), _p(bias), *ptrs, C.byref(p), _p(ws), ws.nbytes if ws is not None else 0, _s()))
+    return Routing(*out) if tables else Routing(out[0], out[1], None, None, None, None, None)
 
 
 def increment(counter):
