@@ -2,10 +2,17 @@
 // a_scale[b, m] * b_scale[n / 128, b] * (A[m, block b] . B[n, block b])), dense and grouped by expert.
 //
 // The scales change along the contraction, so the tensor cores can sum one block only: four MMAs (32 of K each) fill one of four TMEM
-// buffers of BN columns, and while they fill the next ones, the eight warps of the epilogue read it and add it, scaled, to
-// sums in registers (f32; two warps share a TMEM lane quarter, each thread has half a row).  A block of K is one stage of the operand ring: 128 rows
-// x 128 bytes of A, BN x 128 of B.  When the last block is in, the sums go back to TMEM, from where the plain epilogue takes
-// them 16 columns at a time.
+// buffers of BN columns, and while they fill the next ones, eight warps read it and add it, scaled, to sums in registers (f32; two
+// warps share a TMEM lane quarter, a thread has half a row).  A block of K is one stage of the operand ring: 128 rows x 128 bytes of A,
+// BN x 128 of B.  When the last block is in, the sums go back to TMEM, from where the plain epilogue takes them 16 columns at a time.
+//
+// What bounds the main loop is how fast the warps get through their instructions (clocks a block of K, 512 x 2048 x 8192):
+//   - the MMA thread took 366 with divisions by the number of stages and waits asked for when they were due, whatever the width: its loop
+//     counts up, asks for the next stage and buffer before it issues, and is unrolled, since an MMA holds its descriptors' registers until
+//     the tensor core takes it (269 -> 150 - 190 without the sums);
+//   - the warps that sum took 865 with the scales loaded four blocks ahead (a load waits behind the operands, over 1000 clocks), 580 - 690
+//     with 16 warps of half the columns (what every warp does once a block filled the schedulers), and take 330 (64 columns) and 420 (128).
+// 24.5 -> 16.4 us and 28.3 -> 18.6 us at that size.
 //
 // Warp 0 TMA, warp 1 MMA, warps 2-9 sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
 #include <atomic>
@@ -14,7 +21,11 @@
 
 namespace qb {
 
-constexpr int kAccBuffers = 4;
+constexpr int kSumWarps = 8;
+constexpr int kSumThreads = 32 * kSumWarps;
+constexpr int kColGroups = kSumWarps / 4;  // warps that share a TMEM lane quarter, each with its columns
+constexpr int kBlockThreads = 64 + kSumThreads;
+constexpr int kScales = 8;  // blocks whose scales a thread has on their way
 
 struct BlockArgs {
   GemmArgs g;
@@ -28,16 +39,23 @@ struct BlockArgs {
 
 template <int BN>
 struct BlockSmem {
-  static constexpr int kStageBytes = (kBM + BN) * kRowBytes;
+  static constexpr int kStageBytes = (kBM + BN) * kRowBytes;  // a block of K: the rows of A, then those of B
   static constexpr int kSliceBytes = BN == 64 ? kBM * BN * 4 : 0;  // partial sums that the cluster's other K slices push
   static constexpr int kStages = BN == 64 ? 7 : 6;
+  static constexpr int kAccBuffers = 4;  // of a block's products in TMEM
   static constexpr int kSliceOffset = kStages * kStageBytes;
   static constexpr int kBarOffset = kSliceOffset + kSliceBytes;
   static constexpr int kColOffset = kBarOffset + 256;  // per-column scale (unused), bias, gate
   static constexpr int kTopOffset = kColOffset + 3 * BN * 4;
-  static constexpr int kTotal = kTopOffset + 2 * kBM * 4 + 1024;  // + alignment slack
-  static_assert((2 * kStages + 2 * kAccBuffers) * 8 + 32 <= 256 && kTotal <= 227 * 1024, "shared memory of one CTA");
+  static constexpr int kTotal = kTopOffset + kColGroups * kBM * 4 + 1024;  // + alignment slack
+  static_assert((2 * kStages + kAccBuffers) * 8 + 32 <= 256 && kTotal <= 227 * 1024, "shared memory of one CTA");
 };
+
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 
 // d += a * b on two f32 at once
 __device__ __forceinline__ void fma2(float2& d, float ax, float ay, float2 b) {
@@ -50,27 +68,30 @@ __device__ __forceinline__ void fma2(float2& d, float ax, float ay, float2 b) {
 }
 
 template <int BN, bool GROUPED>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kBlockThreads, 1)
 gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_small, const __grid_constant__ CUtensorMap tmB, const BlockArgs args) {
   using L = BlockSmem<BN>;
   constexpr int kStages = L::kStages;
+  constexpr int kAccBuffers = L::kAccBuffers;
   constexpr uint32_t kTmemCols = kAccBuffers * BN;
   constexpr uint32_t kIdesc = umma_idesc(0, 0, kBM, BN);
-  constexpr int kHalf = BN / 2;  // columns of a thread
+  constexpr int kCols = BN / kColGroups;  // columns of a thread
   const GemmArgs& g = args.g;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + L::kBarOffset);
+  // [stage] the MMAs that read the stage are done: it may be filled again, and their products are complete.  (The barrier cannot be a
+  // phase ahead of a warp that sums: the stage's next MMAs come kStages blocks later, behind the sums of the block kAccBuffers before.)
   uint64_t* empty_bar = full_bar + kStages;
-  uint64_t* acc_full = empty_bar + kStages;       // [buffer] a block's products are complete
-  uint64_t* acc_empty = acc_full + kAccBuffers;   // [buffer] the eight warps have read them
+  static_assert(kStages >= kAccBuffers, "see above");
+  uint64_t* acc_empty = empty_bar + kStages;      // [buffer] the warps that sum have read a block's products
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccBuffers);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* drain_flag = abort_flag + 1;  // never set: lets the drain waits below run their own limit
   volatile int* lost_flag = abort_flag + 2;   // set by a CTA of the cluster whose slice is missing
   float* col = reinterpret_cast<float*>(smem + L::kColOffset);
-  float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // [half][row]: largest magnitude of half a row
+  float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // [column group][row]: largest magnitude of a thread's columns
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * BN, m0 = blockIdx.y * kBM, split = blockIdx.z;
@@ -96,10 +117,7 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
-    for (int b = 0; b < kAccBuffers; ++b) {
-      mbar_init(smem_u32(&acc_full[b]), 1);
-      mbar_init(smem_u32(&acc_empty[b]), 8);
-    }
+    for (int b = 0; b < kAccBuffers; ++b) mbar_init(smem_u32(&acc_empty[b]), kColGroups * ((rows + 31) / 32));  // of the warps that have a row
     *abort_flag = 0;
     *drain_flag = 0;
     *lost_flag = 0;
@@ -121,59 +139,64 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if (elect_one()) {
       const CUtensorMap* a_map = small ? &tmA_small : &tmA;
       const int b_row0 = expert * g.N + n0;
+      const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), stage0 = smem_u32(smem);
       // constant weights do not depend on the kernels before this one: their first tiles are on the way while those finish
       const int ahead = !GROUPED && g.b_const ? min(kStages, n_iter) : 0;
       for (int it = 0; it < ahead; ++it) {
-        const uint32_t fb = smem_u32(&full_bar[it]);
-        mbar_arrive_expect_tx(fb, stage_tx);
-        tma_load_2d(smem_u32(smem + it * L::kStageBytes + kBM * kRowBytes), &tmB, fb, (kb0 + it) * 128, b_row0);
+        mbar_arrive_expect_tx(full0 + it * 8, stage_tx);
+        tma_load_2d(stage0 + it * L::kStageBytes + kBM * kRowBytes, &tmB, full0 + it * 8, (kb0 + it) * 128, b_row0);
       }
       if (!GROUPED) grid_dep_wait();
-      for (int it = 0; it < ahead; ++it) tma_load_2d(smem_u32(smem + it * L::kStageBytes), a_map, smem_u32(&full_bar[it]), (kb0 + it) * 128, m0);
-      int issued = ahead;
-      for (int it = ahead; it < n_iter; ++it) {
-        const int s = it % kStages;
-        const uint32_t ph = (it / kStages) & 1;
-        if (!mbar_wait(smem_u32(&empty_bar[s]), ph ^ 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        const uint32_t fb = smem_u32(&full_bar[s]), st = smem_u32(smem + s * L::kStageBytes);
+      for (int it = 0; it < ahead; ++it) tma_load_2d(stage0 + it * L::kStageBytes, a_map, full0 + it * 8, (kb0 + it) * 128, m0);
+      int it = ahead, s = ahead == kStages ? 0 : ahead;
+      uint32_t ph = ahead == kStages ? 0 : 1;  // (a fresh barrier passes for parity 1)
+#pragma unroll 2
+      for (; it < n_iter; ++it) {
+        if (!mbar_wait(empty0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        const uint32_t fb = full0 + s * 8, st = stage0 + s * L::kStageBytes;
         mbar_arrive_expect_tx(fb, stage_tx);
         tma_load_2d(st + kBM * kRowBytes, &tmB, fb, (kb0 + it) * 128, b_row0);
         tma_load_2d(st, a_map, fb, (kb0 + it) * 128, m0);
-        issued = it + 1;
+        if (++s == kStages) { s = 0; ph ^= 1; }
       }
       if (*abort_flag) {
         // Giving up: let the copies already in flight land before this CTA's memory goes away.
-        for (int it = max(0, issued - kStages); it < issued; ++it)
-          mbar_wait(smem_u32(&full_bar[it % kStages]), (it / kStages) & 1, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+        for (int i = max(0, it - kStages); i < it; ++i)
+          mbar_wait(full0 + i % kStages * 8, (i / kStages) & 1, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
       } else {
         // Tail: see the last stage releases land before the CTA can exit.
-        for (int it = max(0, n_iter - kStages); it < n_iter; ++it)
-          if (!mbar_wait(smem_u32(&empty_bar[it % kStages]), (it / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        for (int i = max(0, n_iter - kStages); i < n_iter; ++i)
+          if (!mbar_wait(empty0 + i % kStages * 8, (i / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer: one block of K into one buffer
     if (elect_one()) {
-      bool ok = true;
-      for (int it = 0; it < n_iter && ok; ++it) {
-        const int s = it % kStages, buf = it % kAccBuffers;
-        ok = mbar_wait(smem_u32(&full_bar[s]), (it / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
-        if (ok && it >= kAccBuffers)
-          ok = mbar_wait(smem_u32(&acc_empty[buf]), (it / kAccBuffers - 1) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
-        if (!ok) break;
+      const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), taken0 = smem_u32(acc_empty);
+      const uint64_t desc0 = umma_desc_k_sw128(smem_u32(smem));
+      int s = 0, buf = 0;
+      uint32_t ph = 0, bph = 1;  // (a fresh buffer passes for parity 1)
+      bool landed = false, taken = true;  // what the barriers of this stage and buffer said a block earlier
+#pragma unroll 4
+      for (int it = 0; it < n_iter; ++it) {
+        if (!landed && !mbar_wait(full0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        if (!taken && !mbar_wait(taken0 + buf * 8, bph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
         tc_fence_after();
-        const uint32_t a_addr = smem_u32(smem + s * L::kStageBytes);
-        const uint64_t a_desc = umma_desc_k_sw128(a_addr), b_desc = umma_desc_k_sw128(a_addr + kBM * kRowBytes);
+        const uint64_t a_desc = desc0 + static_cast<uint64_t>(s * (L::kStageBytes >> 4)), b_desc = a_desc + (kBM * kRowBytes >> 4);
+        const uint32_t d = tmem_base + buf * BN, release = empty0 + s * 8;
+        if (++s == kStages) { s = 0; ph ^= 1; }
+        if (++buf == kAccBuffers) { buf = 0; bph ^= 1; }
+        landed = mbar_test_wait(full0 + s * 8, ph);
+        taken = mbar_test_wait(taken0 + buf * 8, bph);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f8(tmem_base + buf * BN, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&empty_bar[s]));
+        for (int k = 0; k < 4; ++k) umma_f8(d, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k > 0 ? 1u : 0u);
         if (it == n_iter - 1 && late(blockIdx.x == gridDim.x - 1 && blockIdx.z == gridDim.z - 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        umma_commit(smem_u32(&acc_full[buf]));  // (not reached: the other warps give up as well)
+        umma_commit(release);  // (not reached: the other warps give up as well)
       }
     }
   } else {
     // ---------------- sums and epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31
-    const int lane_grp = warp & 3, half = (warp - 2) >> 2, et = threadIdx.x - 64;
+    const int lane_grp = warp & 3, group = (warp - 2) >> 2, et = threadIdx.x - 64;
     const int row = lane_grp * 32 + lane, m = m0 + row;
     const bool live = row < rows, busy = lane_grp * 32 < rows;  // this thread's row, any row of this warp
     if (!GROUPED) grid_dep_wait();
@@ -182,19 +205,29 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int slice_rows = kBM / (clustered ? g.splits : 1), slice_row0 = clustered ? split * slice_rows : 0;  // rows this CTA finishes
     const float* as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + m;
     const float* bs = after_wait(args.b_scale) + static_cast<size_t>(expert * ((g.N + 127) / 128) + n0 / 128) * g.kb_total + kb0;
-    float sc[4];  // scales of the next four blocks
-    auto scale_of = [&](int it) { return it < n_iter && live ? as[static_cast<size_t>(it) * g.M] * bs[it] : 0.f; };
+    // The scales of this thread's row and of the tile's columns, loaded kScales blocks ahead: behind the operands' traffic a load takes
+    // over 1000 clocks, as long as four blocks.
+    float sa[kScales], sb[kScales];
+    auto fetch_scales = [&](int j, int it) {
+      sa[j] = sb[j] = 0.f;
+      if (it < n_iter) {
+        if (live) sa[j] = *as;
+        sb[j] = *bs;
+      }
+      as += g.M;
+      ++bs;
+    };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sc[j] = scale_of(j);
+    for (int j = 0; j < kScales; ++j) fetch_scales(j, j);
     // the tile's per-column vectors, and the residuals of the 8-column groups that this thread finishes for the cluster
-    for (int j = et; j < BN; j += 256) {
+    for (int j = et; j < BN; j += kSumThreads) {
       const int n = n0 + j;
       const bool in = n < g.N;
       col[BN + j] = (in && g.bias) ? bf16_bits_to_f32(g.bias[n]) : 0.f;
       col[2 * BN + j] = (in && g.gate) ? bf16_bits_to_f32(g.gate[static_cast<size_t>(m0 / g.rows_per_gate) * g.N + n]) : 0.f;
     }
     uint4 pre[BN / 32][2];
-    if (clustered && one_gate && g.gate != nullptr) {
+    if (clustered && one_gate && g.gate != nullptr && et < 256) {
 #pragma unroll
       for (int k = 0; k < BN / 32; ++k) {
         const int r = et / (BN / 8) + 256 / (BN / 8) * k, mm = m0 + slice_row0 + r, n = n0 + et % (BN / 8) * 8;
@@ -202,58 +235,70 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (r < slice_rows && mm < g.M && n < g.N) pre[k][0] = *reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(mm) * g.N + n);
       }
     }
-    asm volatile("bar.sync 2, 256;" ::: "memory");
+    asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
 
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_grp * 32) << 16) + half * kHalf;
-    float2 acc[kHalf / 2];
+    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_grp * 32) << 16) + group * kCols;
+    float2 acc[kCols / 2];
 #pragma unroll
-    for (int j = 0; j < kHalf / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    bool ok = true;
-    for (int base = 0; base < n_iter && ok; base += kAccBuffers) {
+    for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    // Half of a thread's columns is on its way from TMEM while the other half is added.  The instructions count: with 16 warps of half
+    // the columns, and the scales through shared memory, what a warp does once per block took the schedulers 400 clocks.
+    constexpr int kPart = kCols / 2;
+    uint32_t t[2][kPart];
+    const uint32_t done0 = smem_u32(empty_bar);
+    int ws = 0;
+    uint32_t wph = 0;
+    auto next_block = [&]() {
+      mbar_wait_warp(done0 + ws * 8, wph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+      if (++ws == kStages) { ws = 0; wph ^= 1; }
+      tc_fence_after();
+    };
+    if (busy) {
+      next_block();
+      tmem_ld(taddr, t[0]);
+#pragma unroll 1
+      for (int base = 0; base < n_iter; base += kScales) {
 #pragma unroll
-      for (int j = 0; j < kAccBuffers; ++j) {
-        const int it = base + j;
-        if (it >= n_iter) break;
-        const float s = sc[j];
-        sc[j] = scale_of(it + 4);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(smem_u32(&acc_full[j]), (it / kAccBuffers) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM));
-        if (!ok) break;
-        tc_fence_after();
-        uint32_t t[kHalf / 32][32];
-        if (busy) {
-#pragma unroll
-          for (int c = 0; c < kHalf / 32; ++c) tmem_ld32(taddr + j * BN + c * 32, t[c]);
-          tmem_wait_ld_into(t[0]);
-#pragma unroll
-          for (int c = 1; c < kHalf / 32; ++c) tmem_loaded(t[c]);
-          tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j]));
-        if (busy) {
+        for (int j = 0; j < kScales; ++j) {
+          const int it = base + j;
+          if (it >= n_iter) break;
+          const uint32_t from = taddr + j % kAccBuffers * BN;
+          const float s = sa[j] * sb[j];
           const float2 s2 = make_float2(s, s);
+          fetch_scales(j, it + kScales);
+          tmem_wait_ld_into(t[0]);
+          tmem_ld(from + kPart, t[1]);
 #pragma unroll
-          for (int c = 0; c < kHalf / 32; ++c)
+          for (int q = 0; q < kPart / 2; ++q) fma2(acc[q], __uint_as_float(t[0][2 * q]), __uint_as_float(t[0][2 * q + 1]), s2);
+          tmem_wait_ld_into(t[1]);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j % kAccBuffers]));
+          if (it + 1 < n_iter) {
+            next_block();
+            tmem_ld(taddr + (j + 1) % kAccBuffers * BN, t[0]);
+          }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], __uint_as_float(t[c][2 * i]), __uint_as_float(t[c][2 * i + 1]), s2);
+          for (int q = 0; q < kPart / 2; ++q) fma2(acc[kPart / 2 + q], __uint_as_float(t[1][2 * q]), __uint_as_float(t[1][2 * q + 1]), s2);
         }
       }
     }
+    bool ok = *abort_flag == 0;
     const bool precise = g.c_dtype != QB_BF16;
     if (clustered) {
       if constexpr (BN == 64) {
-        ok = all_of_epilogue(ok);
+        ok = all_of_epilogue<kSumThreads>(ok);
         if (ok) {
           const uint32_t dst = map_to_cta(smem_u32(smem + L::kSliceOffset), row / slice_rows);
 #pragma unroll
-          for (int v = 0; v < kHalf / 4; ++v)
-            st_dsmem_v4(dst + 16 * slice_unit<BN>(split, half * (kHalf / 4) + v, row % slice_rows, slice_rows), __float_as_uint(acc[2 * v].x), __float_as_uint(acc[2 * v].y),
+          for (int v = 0; v < kCols / 4; ++v)
+            st_dsmem_v4(dst + 16 * slice_unit<BN>(split, group * (kCols / 4) + v, row % slice_rows, slice_rows), __float_as_uint(acc[2 * v].x), __float_as_uint(acc[2 * v].y),
                         __float_as_uint(acc[2 * v + 1].x), __float_as_uint(acc[2 * v + 1].y));
         } else if (threadIdx.x == 64) {
           tell_lost<1>(lost_flag, 0, g.splits);
         }
         cluster_sync();  // every slice's share of this CTA's rows has arrived after this barrier (warps 0 and 1 join it below)
-        if (ok && *lost_flag == 0) {
+        if (ok && *lost_flag == 0 && et < 256) {
           const float4* parts = reinterpret_cast<const float4*>(smem + L::kSliceOffset);
           if (precise) finish_slices<BN, true>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
           else finish_slices<BN, false>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
@@ -261,27 +306,26 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
     } else {
       const bool narrow = args.c_scale != nullptr;
-      if (narrow) ok = all_of_epilogue(ok);  // its two halves of a row meet at a barrier
+      if (narrow) ok = all_of_epilogue<kSumThreads>(ok);  // the threads of a row meet at a barrier
       if (ok && busy) {
         // every MMA of the CTA is done (this warp has waited for each block), and a warp reads back what it wrote itself
 #pragma unroll
-        for (int c = 0; c < kHalf / 32; ++c) {
-          uint32_t w[32];
+        for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            w[2 * i] = __float_as_uint(acc[c * 16 + i].x);
-            w[2 * i + 1] = __float_as_uint(acc[c * 16 + i].y);
+          for (int q = 0; q < kPart / 2; ++q) {
+            t[c][2 * q] = __float_as_uint(acc[c * (kPart / 2) + q].x);
+            t[c][2 * q + 1] = __float_as_uint(acc[c * (kPart / 2) + q].y);
           }
-          tmem_st32(taddr + c * 32, w);
+          tmem_st(taddr + c * kPart, t[c]);
         }
         tmem_wait_st();
         const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.C) & 31u) == 0;
         uint8_t* c_row = live ? row_of_c(g, m) : nullptr;
         const uint4* res_row = reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(m) * g.N + n0);
-        const int c0 = half * kHalf;
+        const int c0 = group * kCols;
         uint4 next[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};  // residual of the next turn
         auto fetch = [&](int c) {
-          if (g.gate != nullptr && c < c0 + kHalf && live && n0 + c < g.N) {
+          if (g.gate != nullptr && c < c0 + kCols && live && n0 + c < g.N) {
             next[0] = res_row[c / 8];
             if (n0 + c + 8 < g.N) next[1] = res_row[c / 8 + 1];
           }
@@ -289,7 +333,7 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         fetch(c0);
         float top = 0.f;
 #pragma unroll 1
-        for (int c = c0; c < c0 + kHalf; c += 16) {
+        for (int c = c0; c < c0 + kCols; c += 16) {
           if (n0 + c >= g.N) break;
           uint4 res[2] = {next[0], next[1]};
           uint32_t r[16];
@@ -315,23 +359,26 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
         if (narrow) {
           tmem_wait_st();
-          tops[half * kBM + row] = top;
+          tops[group * kBM + row] = top;
         }
       }
       if constexpr (BN == 128) {
         if (narrow && ok) {
-          asm volatile("bar.sync 2, 256;" ::: "memory");
+          asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
           if (busy) {
-            const float s = block_scale(fmaxf(tops[row], tops[kBM + row]), args.pow2 != 0), inv = __frcp_rn(s);
-            if (live && half == 0) args.c_scale[static_cast<size_t>(n0 / 128) * g.M + m] = s;
+            float top = tops[row];
+#pragma unroll
+            for (int q = 1; q < kColGroups; ++q) top = fmaxf(top, tops[q * kBM + row]);
+            const float s = block_scale(top, args.pow2 != 0), inv = __frcp_rn(s);
+            if (live && group == 0) args.c_scale[static_cast<size_t>(n0 / 128) * g.M + m] = s;
             uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
             const bool wide = g.N % 16 == 0;
 #pragma unroll 1
-            for (int c = half * kHalf; c < (half + 1) * kHalf; c += 16) {
+            for (int c = group * kCols; c < (group + 1) * kCols; c += 16) {
               const int n = n0 + c;
               if (n >= g.N) break;
               uint32_t r[16], w[4];
-              tmem_ld16(taddr + c - half * kHalf, r);
+              tmem_ld16(taddr + c - group * kCols, r);
               tmem_wait_ld_into(r);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
@@ -408,7 +455,7 @@ static int32_t launch_blocks(const CUtensorMap& tmA, const CUtensorMap& tmA_smal
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.blockDim = dim3(kBlockThreads);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];

@@ -195,16 +195,17 @@ __device__ __forceinline__ void tell_lost(volatile int* lost_flag, int rank, int
 // The same for slices through the workspace: what such a CTA adds to the tile's counter, whose lower half counts the tickets.
 constexpr int kLostTicket = 1 << 16;
 
-// Whether `ok` holds for all 256 epilogue threads (a barrier of theirs).
+// Whether `ok` holds for all epilogue threads (a barrier of theirs).
+template <int kThreads = 256>
 __device__ __forceinline__ bool all_of_epilogue(bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 q, %1, 0;\n\t"
-      "bar.red.and.pred p, 2, 256, q;\n\t"
+      "bar.red.and.pred p, 2, %2, q;\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(r)
-      : "r"(ok ? 1 : 0)
+      : "r"(ok ? 1 : 0), "n"(kThreads)
       : "memory");
   return r != 0;
 }
