@@ -24,8 +24,15 @@ namespace qb {
 constexpr int kSumWarps = 8;
 constexpr int kSumThreads = 32 * kSumWarps;
 constexpr int kColGroups = kSumWarps / 4;  // warps that share a TMEM lane quarter, each with its columns
-constexpr int kBlockThreads = 64 + kSumThreads;
-constexpr int kScales = 8;  // blocks whose scales a thread has on their way
+
+// 256 columns: a thread has 128 sums beside what is on its way.  The control warps are a warpgroup of their own then, which hands
+// registers over (setmaxnreg): an increase waits until that many are free, so the shares have to fit what the launch was given.
+constexpr int kWideThreads = 384, kWideLaunchRegs = 168, kWideCtrlRegs = 56, kWideSumRegs = 224;
+static_assert(128 * kWideCtrlRegs + kSumThreads * kWideSumRegs <= kWideThreads * kWideLaunchRegs, "register budget of the CTA");
+template <int BN>
+constexpr int kFirstSumWarp = BN == 256 ? 4 : 2;
+template <int BN>
+constexpr int kBlockThreads = 32 * kFirstSumWarp<BN> + kSumThreads;
 
 struct BlockArgs {
   GemmArgs g;
@@ -41,8 +48,8 @@ template <int BN>
 struct BlockSmem {
   static constexpr int kStageBytes = (kBM + BN) * kRowBytes;  // a block of K: the rows of A, then those of B
   static constexpr int kSliceBytes = BN == 64 ? kBM * BN * 4 : 0;  // partial sums that the cluster's other K slices push
-  static constexpr int kStages = BN == 64 ? 7 : 6;
-  static constexpr int kAccBuffers = 4;  // of a block's products in TMEM
+  static constexpr int kStages = BN == 64 ? 7 : BN == 128 ? 6 : 4;
+  static constexpr int kAccBuffers = BN == 256 ? 2 : 4;  // of a block's products in TMEM
   static constexpr int kSliceOffset = kStages * kStageBytes;
   static constexpr int kBarOffset = kSliceOffset + kSliceBytes;
   static constexpr int kColOffset = kBarOffset + 256;  // per-column scale (unused), bias, gate
@@ -68,11 +75,12 @@ __device__ __forceinline__ void fma2(float2& d, float ax, float ay, float2 b) {
 }
 
 template <int BN, bool GROUPED>
-__global__ void __launch_bounds__(kBlockThreads, 1)
+__global__ void __launch_bounds__(kBlockThreads<BN>, 1)
 gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA_small, const __grid_constant__ CUtensorMap tmB, const BlockArgs args) {
   using L = BlockSmem<BN>;
   constexpr int kStages = L::kStages;
-  constexpr int kAccBuffers = L::kAccBuffers;
+  constexpr int kAccBuffers = L::kAccBuffers, kW0 = kFirstSumWarp<BN>;
+  constexpr int kScales = BN == 256 ? 4 : 8;  // blocks whose scales a thread has on their way
   constexpr uint32_t kTmemCols = kAccBuffers * BN;
   constexpr uint32_t kIdesc = umma_idesc(0, 0, kBM, BN);
   constexpr int kCols = BN / kColGroups;  // columns of a thread
@@ -91,7 +99,7 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   volatile int* drain_flag = abort_flag + 1;  // never set: lets the drain waits below run their own limit
   volatile int* lost_flag = abort_flag + 2;   // set by a CTA of the cluster whose slice is missing
   float* col = reinterpret_cast<float*>(smem + L::kColOffset);
-  float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // [column group][row]: largest magnitude of a thread's columns
+  float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // 128 columns: [column group][row], largest magnitude of a thread's columns
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n0 = blockIdx.x * BN, m0 = blockIdx.y * kBM, split = blockIdx.z;
@@ -134,6 +142,7 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   if (!GROUPED) grid_dep_launch();
 
+  if (BN == 256 && warp < kW0) setmaxnreg_dec<kWideCtrlRegs>();
   if (warp == 0) {
     // ---------------- TMA producer
     if (elect_one()) {
@@ -194,28 +203,26 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         umma_commit(release);  // (not reached: the other warps give up as well)
       }
     }
-  } else {
+  } else if (warp >= kW0) {
     // ---------------- sums and epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31
-    const int lane_grp = warp & 3, group = (warp - 2) >> 2, et = threadIdx.x - 64;
+    if (BN == 256) setmaxnreg_inc<kWideSumRegs>();
+    const int lane_grp = warp & 3, group = (warp - kW0) >> 2, et = threadIdx.x - 32 * kW0;
     const int row = lane_grp * 32 + lane, m = m0 + row;
     const bool live = row < rows, busy = lane_grp * 32 < rows;  // this thread's row, any row of this warp
     if (!GROUPED) grid_dep_wait();
     const int m_last = m0 + rows - 1;
     const bool one_gate = g.gate == nullptr || m0 / g.rows_per_gate == m_last / g.rows_per_gate;
     const int slice_rows = kBM / (clustered ? g.splits : 1), slice_row0 = clustered ? split * slice_rows : 0;  // rows this CTA finishes
-    const float* as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + m;
-    const float* bs = after_wait(args.b_scale) + static_cast<size_t>(expert * ((g.N + 127) / 128) + n0 / 128) * g.kb_total + kb0;
-    // The scales of this thread's row and of the tile's columns, loaded kScales blocks ahead: behind the operands' traffic a load takes
-    // over 1000 clocks, as long as four blocks.
+    // The scales of this thread's row and of its columns, loaded kScales blocks ahead: behind the operands' traffic a load takes over
+    // 1000 clocks, as long as four blocks of 64 columns.  (Rows and blocks past the last are read as the last, without a branch.)
+    const int nb = (g.N + 127) / 128;  // (256 columns: a thread's 128 are one block's)
+    const float* as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + min(m, m_last);
+    const float* bs = after_wait(args.b_scale) + static_cast<size_t>(expert * nb + min(n0 / 128 + (BN == 256 ? group : 0), nb - 1)) * g.kb_total + kb0;
     float sa[kScales], sb[kScales];
     auto fetch_scales = [&](int j, int it) {
-      sa[j] = sb[j] = 0.f;
-      if (it < n_iter) {
-        if (live) sa[j] = *as;
-        sb[j] = *bs;
-      }
-      as += g.M;
-      ++bs;
+      const unsigned at = min(it, n_iter - 1);
+      sa[j] = as[static_cast<size_t>(at) * static_cast<unsigned>(g.M)];
+      sb[j] = bs[at];
     };
 #pragma unroll
     for (int j = 0; j < kScales; ++j) fetch_scales(j, j);
@@ -241,9 +248,8 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     float2 acc[kCols / 2];
 #pragma unroll
     for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    // Half of a thread's columns is on its way from TMEM while the other half is added.  The instructions count: with 16 warps of half
-    // the columns, and the scales through shared memory, what a warp does once per block took the schedulers 400 clocks.
-    constexpr int kPart = kCols / 2;
+    // Of a thread's columns one part is on its way from TMEM while the last one is added.
+    constexpr int kPart = kCols / 2 < 32 ? kCols / 2 : 32, kParts = kCols / kPart;
     uint32_t t[2][kPart];
     const uint32_t done0 = smem_u32(empty_bar);
     int ws = 0;
@@ -266,20 +272,23 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           const float s = sa[j] * sb[j];
           const float2 s2 = make_float2(s, s);
           fetch_scales(j, it + kScales);
-          tmem_wait_ld_into(t[0]);
-          tmem_ld(from + kPart, t[1]);
 #pragma unroll
-          for (int q = 0; q < kPart / 2; ++q) fma2(acc[q], __uint_as_float(t[0][2 * q]), __uint_as_float(t[0][2 * q + 1]), s2);
-          tmem_wait_ld_into(t[1]);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j % kAccBuffers]));
-          if (it + 1 < n_iter) {
-            next_block();
-            tmem_ld(taddr + (j + 1) % kAccBuffers * BN, t[0]);
+          for (int c = 0; c < kParts; ++c) {
+            tmem_wait_ld_into(t[c & 1]);
+            if (c + 1 < kParts) {
+              tmem_ld(from + (c + 1) * kPart, t[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j % kAccBuffers]));
+              if (it + 1 < n_iter) {
+                next_block();
+                tmem_ld(taddr + (j + 1) % kAccBuffers * BN, t[0]);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < kPart / 2; ++q) fma2(acc[c * (kPart / 2) + q], __uint_as_float(t[c & 1][2 * q]), __uint_as_float(t[c & 1][2 * q + 1]), s2);
           }
-#pragma unroll
-          for (int q = 0; q < kPart / 2; ++q) fma2(acc[kPart / 2 + q], __uint_as_float(t[1][2 * q]), __uint_as_float(t[1][2 * q + 1]), s2);
         }
       }
     }
@@ -306,17 +315,18 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
     } else {
       const bool narrow = args.c_scale != nullptr;
-      if (narrow) ok = all_of_epilogue<kSumThreads>(ok);  // the threads of a row meet at a barrier
+      float row_top = 0.f;
+      if (BN == 128 && narrow) ok = all_of_epilogue<kSumThreads>(ok);  // the two threads of a row's 128 columns meet at a barrier
       if (ok && busy) {
         // every MMA of the CTA is done (this warp has waited for each block), and a warp reads back what it wrote itself
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kParts; ++c) {
 #pragma unroll
           for (int q = 0; q < kPart / 2; ++q) {
-            t[c][2 * q] = __float_as_uint(acc[c * (kPart / 2) + q].x);
-            t[c][2 * q + 1] = __float_as_uint(acc[c * (kPart / 2) + q].y);
+            t[c & 1][2 * q] = __float_as_uint(acc[c * (kPart / 2) + q].x);
+            t[c & 1][2 * q + 1] = __float_as_uint(acc[c * (kPart / 2) + q].y);
           }
-          tmem_st(taddr + c * kPart, t[c]);
+          tmem_st(taddr + c * kPart, t[c & 1]);
         }
         tmem_wait_st();
         const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.C) & 31u) == 0;
@@ -359,18 +369,18 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
         if (narrow) {
           tmem_wait_st();
-          tops[group * kBM + row] = top;
+          if (BN == 128) tops[group * kBM + row] = top;
+          row_top = top;
         }
       }
-      if constexpr (BN == 128) {
+      if constexpr (BN >= 128) {
         if (narrow && ok) {
-          asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
+          if (BN == 128) asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
           if (busy) {
-            float top = tops[row];
-#pragma unroll
-            for (int q = 1; q < kColGroups; ++q) top = fmaxf(top, tops[q * kBM + row]);
-            const float s = block_scale(top, args.pow2 != 0), inv = __frcp_rn(s);
-            if (live && group == 0) args.c_scale[static_cast<size_t>(n0 / 128) * g.M + m] = s;
+            if (BN == 128) row_top = fmaxf(tops[row], tops[kBM + row]);
+            const float s = block_scale(row_top, args.pow2 != 0), inv = __frcp_rn(s);
+            const int block = n0 / 128 + (BN == 256 ? group : 0);
+            if (live && (BN == 256 ? block < nb : group == 0)) args.c_scale[static_cast<size_t>(block) * g.M + m] = s;
             uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
             const bool wide = g.N % 16 == 0;
 #pragma unroll 1
@@ -419,11 +429,11 @@ struct BlockPlan {
 static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
   const int kb_total = (p.K + 127) / 128, sms = num_sms();
   BlockPlan best{128, 1, kb_total, kb_total};
-  if (p.c_dtype == QB_E4M3) return best;  // a group of 128 results is one tile's
   double best_cost = 1e30;
-  for (int bn = 64; bn <= 128; bn += 64) {
+  for (int bn = 64; bn <= 256; bn *= 2) {
     if (p.tile_n != 0 && p.tile_n != bn) continue;
-    if (bn == 128 && p.tile_n == 0 && p.N <= 64) continue;
+    if (p.c_dtype == QB_E4M3 && bn == 64) continue;  // a group of 128 results is one tile's
+    if (bn > 64 && p.tile_n == 0 && p.N <= bn / 2 && !(p.c_dtype == QB_E4M3 && bn == 128)) continue;
     for (int s = 1; s <= (bn == 64 ? 8 : 1); s *= 2) {
       if (p.split_k != 0 && p.split_k != s) continue;
       const int kbps = (kb_total + s - 1) / s;
@@ -431,8 +441,8 @@ static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
       const long tiles = static_cast<long>(row_tiles) * ((p.N + bn - 1) / bn);
       const long slots = s == 4 ? 33 : s == 8 ? 15 : sms / s;  // clusters that run at once
       const long rounds = (tiles + slots - 1) / slots;
-      const double body = kbps * (bn == 64 ? 150.0 : 200.0);
-      double cost = 3500.0 + body + (rounds - 1) * (body + 2500.0);
+      const double body = kbps * (bn == 64 ? 165.0 : bn == 128 ? 215.0 : 300.0);
+      double cost = 3500.0 + bn * 4.0 + body + (rounds - 1) * (body + 2500.0 + bn * 4.0);
       if (s > 1) cost += 300.0 + 12.0 * tiles * s;
       if (cost < best_cost) {
         best_cost = cost;
@@ -451,11 +461,14 @@ static int32_t launch_blocks(const CUtensorMap& tmA, const CUtensorMap& tmA_smal
   QB_CUDA_OK(cudaGetDevice(&dev));
   if (dev >= 64 || (configured.load(std::memory_order_relaxed) >> dev & 1) == 0) {
     QB_CUDA_OK(cudaFuncSetAttribute(gemm_blocks_kernel<BN, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal));
+    cudaFuncAttributes fa;
+    QB_CUDA_OK(cudaFuncGetAttributes(&fa, gemm_blocks_kernel<BN, GROUPED>));
+    QB_REQUIRE(BN != 256 || fa.numRegs >= kWideLaunchRegs, QB_ERR_UNSUPPORTED, "gemm_blocks: built with %d registers a thread, %d needed", fa.numRegs, kWideLaunchRegs);
     if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kBlockThreads);
+  cfg.blockDim = dim3(kBlockThreads<BN>);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -485,7 +498,7 @@ static int32_t validate_blocks(const qb_gemm_blocks_params* p) {
   QB_REQUIRE(p->K % 16 == 0, QB_ERR_ALIGN, "gemm_blocks: K = %d must be a multiple of 16", p->K);
   QB_REQUIRE(p->N % 8 == 0, QB_ERR_ALIGN, "gemm_blocks: N = %d must be a multiple of 8", p->N);
   QB_REQUIRE(p->activation == 0 || p->activation == 1, QB_ERR_INVALID_ARG, "gemm_blocks: activation %d", p->activation);
-  QB_REQUIRE(p->tile_n == 0 || p->tile_n == 64 || p->tile_n == 128, QB_ERR_INVALID_ARG, "gemm_blocks: tile_n %d", p->tile_n);
+  QB_REQUIRE(p->tile_n == 0 || p->tile_n == 64 || p->tile_n == 128 || p->tile_n == 256, QB_ERR_INVALID_ARG, "gemm_blocks: tile_n %d", p->tile_n);
   QB_REQUIRE(p->split_k >= 0 && p->split_k <= 8, QB_ERR_INVALID_ARG, "gemm_blocks: split_k %d", p->split_k);
   QB_REQUIRE(p->M <= 65535 * kBM, QB_ERR_INVALID_ARG, "gemm_blocks: %d rows", p->M);
   return QB_OK;
@@ -538,8 +551,8 @@ static int32_t blocks_run(const void* A, const void* B, const float* a_scale, co
   rc = make_tmap_2d_sw(&tmB, B, 1, static_cast<uint64_t>(p->N) * n_experts, p->K, pl.bn, 128, 128);
   if (rc != QB_OK) return rc;
   const dim3 grid((p->N + pl.bn - 1) / pl.bn, row_tiles, pl.splits);
-  if (grouped) return pl.bn == 128 ? launch_blocks<128, true>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, true>(tmA, tmA_small, tmB, a, grid, st);
-  return pl.bn == 128 ? launch_blocks<128, false>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, false>(tmA, tmA_small, tmB, a, grid, st);
+  if (grouped) return pl.bn == 256 ? launch_blocks<256, true>(tmA, tmA_small, tmB, a, grid, st) : pl.bn == 128 ? launch_blocks<128, true>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, true>(tmA, tmA_small, tmB, a, grid, st);
+  return pl.bn == 256 ? launch_blocks<256, false>(tmA, tmA_small, tmB, a, grid, st) : pl.bn == 128 ? launch_blocks<128, false>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, false>(tmA, tmA_small, tmB, a, grid, st);
 }
 
 }  // namespace qb

@@ -6,18 +6,21 @@
 //   the kept groups, then the top k of c inside them (equal values: the lower index first)      w = s / sum of the chosen s * factor
 //
 // A choice compares numbers that may lie next to one another, so it is made on what the formula says and not on a rounding of it:
-// where c grows with l alone (no bias, groups by their best one) on the logits themselves, else on c in 64 bits.  Weights are f32.
+// where c grows with l alone (no bias, groups by their best one) on the logits themselves, else on c in 32 bits as long as what it
+// compares lies apart by more than those are off, and in 64 bits for a token where it does not.  Weights are f32.
 //
 // A warp takes a token; its lanes hold P consecutive experts each.  The tables need, for every choice, how many earlier tokens chose
 // the same expert: a block's tokens are a 64-bit mask per expert (rank = set bits below the token), and blocks are joined by the
-// counts that each leaves in the workspace.  Up to 64 tokens one block does all in one launch.
+// counts (a byte each) that they leave in the workspace.  Up to 64 tokens one block does all in one launch.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace qb {
 
 constexpr int kRouteMaxExperts = 512, kRouteMaxGroups = 32, kRouteMaxTopK = 32;
 constexpr int kRouteTokens = 64;    // tokens of a block
-constexpr int kRouteThreads = 512;  // one thread per expert in the scan
+constexpr int kRouteThreads = 1024;
 constexpr int kRouteTile = 128;     // row tile of the grouped product
 constexpr size_t kRouteWsOffset = 64u << 10;  // the area in front belongs to the GEMM's counters
 
@@ -29,7 +32,9 @@ struct RouteArgs {
   int *experts, *slot_token, *tile_expert, *tile_rows, *token_slot;
   float *weights, *slot_weight;
   int n_tiles;
-  int* counts;  // [block][E]
+  uint8_t* counts;  // [block][E rounded up to 4]
+  int vec, vec_bias;  // rows of logits, and the bias, are whole 16-byte vectors
+  int regular;  // no groups, or groups of whole lanes, a power of two of them
 };
 
 // Unsigned keys in the order of the values; 0 is kept for what cannot be chosen, NaN comes next.
@@ -52,94 +57,30 @@ __device__ __forceinline__ V lowest() {
   return sizeof(V) == 8 ? static_cast<V>(__longlong_as_double(0xfff0000000000000ll)) : static_cast<V>(__uint_as_float(0xff800000u));
 }
 
-// One token: lane j < top_k returns its j-th choice and weight.  V: what the choice compares (float: the logits; double: scores).
+// The choice of one token among the values c of its lanes' experts: lane j < top_k receives the j-th expert.  Exact, and the slow way:
+// up to 3000 instructions a token.
 template <int P, typename V>
-__device__ __forceinline__ void choose(const RouteArgs& a, int t, V* scratch, int& my_expert, float& my_weight) {
+__device__ __noinline__ int select_exact(const RouteArgs& a, const V (&c)[P], V* scratch) {
   const int lane = threadIdx.x & 31, e0 = lane * P;
-  float l[P];
-  const size_t at = static_cast<size_t>(t) * a.E + e0;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    l[i] = __uint_as_float(0xff800000u);
-    if (e0 + i < a.E) l[i] = a.f32 ? static_cast<const float*>(a.logits)[at + i] : bf16_bits_to_f32(static_cast<const uint16_t*>(a.logits)[at + i]);
-  }
-  // softmax: the largest logit (0 for a row that has none) and the sum
-  float top = 0.f, total = 1.f;
-  V c[P];
-  if (!a.sigmoid) {
-    top = l[0];
-#pragma unroll
-    for (int i = 1; i < P; ++i) top = fmaxf(top, l[i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top == __uint_as_float(0xff800000u)) top = 0.f;
-  }
-  if constexpr (sizeof(V) == 8) {
-    if (a.sigmoid) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) c[i] = 1.0 / (1.0 + exp(-static_cast<double>(l[i])));
-    } else {
-      double sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        c[i] = exp(static_cast<double>(l[i]) - static_cast<double>(top));
-        sum += c[i];
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      total = static_cast<float>(sum);
-      const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
-#pragma unroll
-      for (int i = 0; i < P; ++i) c[i] *= inv;
-    }
-    if (a.bias != nullptr) {
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (e0 + i < a.E) c[i] += static_cast<double>(a.bias[e0 + i]);
-    }
-  } else {
-    if (!a.sigmoid && !a.renorm) {
-      total = 0.f;
-#pragma unroll
-      for (int i = 0; i < P; ++i) total += expf(l[i] - top);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) c[i] = l[i];
-  }
   unsigned kept = 0xffffffffu;  // groups
   const int size = a.E / a.groups;
   if (a.groups > 1) {
     V best = lowest<V>(), second = lowest<V>();
-    auto take = [&](V v) {
-      if (v > best) {
-        second = best;
-        best = v;
-      } else if (v > second) {
-        second = v;
-      }
-    };
-    const int lanes = size / P;  // of a group
-    if (size % P == 0 && (lanes & (lanes - 1)) == 0) {
 #pragma unroll
-      for (int i = 0; i < P; ++i) take(c[i]);
-      for (int o = 1; o < lanes; o <<= 1) {
-        const V b = __shfl_xor_sync(0xffffffffu, best, o), s = __shfl_xor_sync(0xffffffffu, second, o);
-        take(b);
-        if (s > second) second = s;
+    for (int i = 0; i < P; ++i)
+      if (e0 + i < a.E) scratch[e0 + i] = c[i];
+    __syncwarp();
+    if (lane < a.groups)
+      for (int i = 0; i < size; ++i) {
+        const V v = scratch[lane * size + i];
+        if (v > best) {
+          second = best;
+          best = v;
+        } else if (v > second) {
+          second = v;
+        }
       }
-      best = __shfl_sync(0xffffffffu, best, lane * lanes & 31);
-      second = __shfl_sync(0xffffffffu, second, lane * lanes & 31);
-    } else {
-#pragma unroll
-      for (int i = 0; i < P; ++i)
-        if (e0 + i < a.E) scratch[e0 + i] = c[i];
-      __syncwarp();
-      if (lane < a.groups)
-        for (int i = 0; i < size; ++i) take(scratch[lane * size + i]);
-      __syncwarp();
-    }
+    __syncwarp();
     auto key = order_key(a.top == 2 ? best + second : best);
     if (lane >= a.groups) key = 0;
     int rank = 0;
@@ -155,35 +96,253 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, V* scratch, in
     const int e = e0 + i;
     key[i] = e < a.E && (a.groups == 1 || (kept >> (e / size) & 1u)) ? order_key(c[i]) : 0;
   }
-  my_expert = 0;
-  float my_logit = 0.f;
+  int mine = 0;
   for (int j = 0; j < a.top_k; ++j) {
     auto k = key[0];
-    int at_i = 0;
-    float v = l[0];
+    int at = 0;
 #pragma unroll
     for (int i = 1; i < P; ++i)
       if (key[i] > k) {
         k = key[i];
-        at_i = i;
-        v = l[i];
+        at = i;
       }
     const auto most = warp_max(k);
     const int who = __ffs(__ballot_sync(0xffffffffu, k == most)) - 1;
-    const int e = __shfl_sync(0xffffffffu, e0 + at_i, who);
-    v = __shfl_sync(0xffffffffu, v, who);
-    if (lane == j) {
-      my_expert = e;
-      my_logit = v;
-    }
+    const int e = __shfl_sync(0xffffffffu, e0 + at, who);
+    if (lane == j) mine = e;
     if (lane == who) {
 #pragma unroll
       for (int i = 0; i < P; ++i)
-        if (i == at_i) key[i] = 0;
+        if (i == at) key[i] = 0;
+    }
+  }
+  return mine;
+}
+
+// The same on values in 32 bits: a lane's experts become keys whose low bits hold their place in the lane, sorted once, and a round takes
+// the largest head.  kMargin: the values are off by less than 2^-20 of max(1, their size) each, low bits included (an exponential
+// of 2 ulp, a sum of at most 20 roundings, a quotient, the bias); without, they are exact but for the low bits.  What the whole warp learns:
+// kFound, kOrder (with kMargin: the choice is among the first top_k + 1, which lanes 0 .. top_k hold, but some of them lie within
+// 2^-18 of one another), or kOpen (too close for that, or equal with low bits lost: select_exact has to choose).
+enum Selected { kFound, kOrder, kOpen };
+template <int P, bool kMargin>
+__device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float (&c)[P], bool lossless, int& mine) {
+  constexpr uint32_t kLow = P > 8 ? 15u : 7u;
+  const int lane = threadIdx.x & 31, e0 = lane * P;
+  uint32_t key[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    uint32_t k = order_key(c[i]);
+    if (c[i] != c[i]) k = kLow + 1;
+    key[i] = e0 + i < a.E ? (k & ~kLow) | (kLow - i) : 0u;
+  }
+  auto value = [](uint32_t k) {
+    k &= ~kLow;
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+  };
+  auto apart = [](float hi, float lo) { return hi - lo > 0x1p-18f * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo))); };
+#pragma unroll
+  for (int size = 2; size <= P; size *= 2)  // descending, by a bitonic network
+#pragma unroll
+    for (int d = size / 2; d > 0; d /= 2)
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if ((i & d) == 0) {
+          const bool down = (i & size) == 0 || size == P;
+          const uint32_t hi = max(key[i], key[i + d]), lo = min(key[i], key[i + d]);
+          key[i] = down ? hi : lo;
+          key[i + d] = down ? lo : hi;
+        }
+  bool fine = true;
+  if (a.groups > 1) {
+    const int lanes = a.E / a.groups / P;  // of a group: a power of two
+    float best = value(key[0]), second = P > 1 ? value(key[P > 1 ? 1 : 0]) : __uint_as_float(0xff800000u);
+    for (int o = 1; o < lanes; o <<= 1) {
+      const float b = __shfl_xor_sync(0xffffffffu, best, o), s = __shfl_xor_sync(0xffffffffu, second, o);
+      second = fmaxf(fminf(best, b), fmaxf(second, s));
+      best = fmaxf(best, b);
+    }
+    const float score = a.top == 2 ? best + second : best;  // of this lane's group
+    uint32_t open = lane * P < a.E ? order_key(score) : 0u;
+    bool mine_kept = false;
+    float last = 0.f;
+    for (int j = 0; j <= a.kept; ++j) {  // (kept < groups)
+      const uint32_t most = __reduce_max_sync(0xffffffffu, open);
+      const int who = __ffs(__ballot_sync(0xffffffffu, open == most)) - 1;
+      const float x = __uint_as_float((most & 0x80000000u) ? most ^ 0x80000000u : ~most);
+      if (j == a.kept) {
+        fine = kMargin ? apart(last, x) : lossless || last != x;
+        break;
+      }
+      last = x;
+      if (lane / lanes == who / lanes) {
+        mine_kept = true;
+        open = 0u;
+      }
+    }
+    if (!mine_kept) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) key[i] = 0u;
+    }
+  }
+  const int left = a.groups == 1 ? a.E : a.kept * (a.E / a.groups);
+  // top_k choices and the next one or two, as far as there are lanes and experts for them; lane j keeps the j-th and its key
+  const int rounds = min(min(a.top_k + (kMargin ? 2 : 1), left), 32);
+  mine = 0;
+  uint32_t got = 0u;
+  for (int j = 0; j < rounds; ++j) {
+    const uint32_t head = key[0] & ~kLow, most = __reduce_max_sync(0xffffffffu, head);
+    const int who = __ffs(__ballot_sync(0xffffffffu, head == most)) - 1;
+    const int e = __shfl_sync(0xffffffffu, e0 + static_cast<int>(kLow - (key[0] & kLow)), who);
+    if (lane == j) {
+      mine = e;
+      got = most;
+    }
+    if (lane == who) {
+#pragma unroll
+      for (int i = 0; i + 1 < P; ++i) key[i] = key[i + 1];
+      key[P - 1] = 0u;
+    }
+  }
+  const int k = a.top_k;
+  const uint32_t next = __shfl_down_sync(0xffffffffu, got, 1), second = __shfl_down_sync(0xffffffffu, got, 2);
+  if (!kMargin) {
+    const bool same = __any_sync(0xffffffffu, lane < k && lane + 1 < rounds && got == next);
+    if (!lossless && (same || (left > k && rounds <= k))) fine = false;
+    return fine ? kFound : kOpen;
+  }
+  const bool close = __any_sync(0xffffffffu, lane < k && lane + 1 < rounds && !apart(value(got), value(next)));
+  // the last choice against the one behind the next: else that might be among the top k
+  const bool far = !__any_sync(0xffffffffu, lane == k - 1 && lane + 2 < rounds && !apart(value(got), value(second)));
+  if (left > k && rounds <= k) return kOpen;  // the 32nd choice has no lane to be compared with
+  if (!close) return fine ? kFound : kOpen;
+  return fine && far && rounds > k && (rounds == k + 2 || left == k + 1) ? kOrder : kOpen;
+}
+
+// P consecutive values of a row as f32; `fill` past E.
+template <int P>
+__device__ __forceinline__ void load_row(const void* row, bool f32, bool vec, int e0, int E, float fill, float (&v)[P]) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = fill;
+  if constexpr (P >= 4) {
+    if (vec) {  // rows are whole 16-byte vectors
+      if (f32) {
+#pragma unroll
+        for (int i = 0; i < P; i += 4)
+          if (e0 + i < E) {
+            const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + e0 + i);
+            v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w;
+          }
+        return;
+      }
+      if constexpr (P >= 8) {
+#pragma unroll
+        for (int i = 0; i < P; i += 8)
+          if (e0 + i < E) {
+            const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + e0 + i);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              v[i + 2 * q] = bf16lo(w[q]);
+              v[i + 2 * q + 1] = bf16hi(w[q]);
+            }
+          }
+        return;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (e0 + i < E) v[i] = f32 ? static_cast<const float*>(row)[e0 + i] : bf16_bits_to_f32(static_cast<const uint16_t*>(row)[e0 + i]);
+}
+
+__device__ __forceinline__ float logit_at(const RouteArgs& a, const uint8_t* row, int e) {
+  return a.f32 ? reinterpret_cast<const float*>(row)[e] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[e]);
+}
+
+// One token: lane j < top_k returns its j-th choice and weight.  kScores: the choice is on c, else on the logits.
+template <int P, bool kScores>
+__device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratch, int& my_expert, float& my_weight) {
+  const int lane = threadIdx.x & 31, e0 = lane * P;
+  const float none = __uint_as_float(0xff800000u);
+  const uint8_t* row = static_cast<const uint8_t*>(a.logits) + static_cast<size_t>(t) * a.E * (a.f32 ? 4 : 2);
+  float l[P];
+  load_row<P>(row, a.f32 != 0, a.vec != 0, e0, a.E, none, l);
+  // softmax: the largest logit (0 for a row that has none) and the sum
+  float top = 0.f, total = 1.f;
+  if (!a.sigmoid) {
+    top = l[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i) top = fmaxf(top, l[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == none) top = 0.f;
+    if (kScores || !a.renorm) {
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) total += expf(l[i] - top);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+  }
+  if (!kScores) {
+    if (!a.regular || select_fast<P, false>(a, l, a.f32 == 0, my_expert) != kFound) my_expert = select_exact<P, float>(a, l, reinterpret_cast<float*>(scratch));
+  } else {
+    Selected found = kOpen;
+    if (a.regular) {
+      float c[P];
+      const float by = total == 0.f ? 0.f : 1.f / total;
+      if (a.bias != nullptr) load_row<P>(a.bias, true, a.vec_bias != 0, e0, a.E, 0.f, c);
+      else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) c[i] = 0.f;
+      }
+      // (|e^x| (2 + 1.16 |x|) 2^-24, what __expf may be off, is largest at small x: 2^-22)
+#pragma unroll
+      for (int i = 0; i < P; ++i) c[i] += a.sigmoid ? __fdividef(1.f, 1.f + __expf(-l[i])) : __expf(l[i] - top) * by;
+      found = select_fast<P, true>(a, c, false, my_expert);
+    }
+    if (found != kFound) {
+      double sum = 0.0;
+      if (!a.sigmoid) {
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) sum += exp(static_cast<double>(l[i]) - static_cast<double>(top));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      const double inv = a.sigmoid || sum == 0.0 ? 0.0 : 1.0 / sum;
+      auto score = [&](float x, int e) {
+        const double s = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - static_cast<double>(top)) * inv;
+        return a.bias != nullptr ? s + static_cast<double>(a.bias[e]) : s;
+      };
+      if (found == kOrder) {  // the candidates in 64 bits, each by the lane that holds it
+        const int n = a.top_k + 1;
+        uint64_t key = 0;
+        if (lane < n) key = order_key(score(logit_at(a, row, my_expert), my_expert));
+        int rank = 0, sorted = 0;
+        for (int i = 0; i < n; ++i) {
+          const uint64_t k = __shfl_sync(0xffffffffu, key, i);
+          const int e = __shfl_sync(0xffffffffu, my_expert, i);
+          rank += k > key || (k == key && e < my_expert);
+        }
+        for (int i = 0; i < n; ++i) {
+          const int e = __shfl_sync(0xffffffffu, my_expert, i);
+          if (__shfl_sync(0xffffffffu, rank, i) == lane) sorted = e;
+        }
+        my_expert = sorted;
+      } else {
+        double d[P];
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) d[i] = e0 + i < a.E ? score(l[i], e0 + i) : 0.0;
+        my_expert = select_exact<P, double>(a, d, scratch);
+      }
     }
   }
   float s = 0.f;
-  if (lane < a.top_k) s = a.sigmoid ? 1.f / (1.f + expf(-my_logit)) : expf(my_logit - top);
+  if (lane < a.top_k) {
+    const float x = logit_at(a, row, my_expert);
+    s = a.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - top);
+  }
   float by = total;
   if (a.renorm) {
     by = s;
@@ -199,7 +358,7 @@ struct RouteShared {
   int warp_sum[kRouteThreads / 32];
 };
 
-// The tables of the block's tokens, and the tiles blockIdx.x, blockIdx.x + gridDim.x, ... of all.  mask, total and before are in place.
+// The tables of the block's tokens, and its share of the rest.  mask, total and before are in place.
 __device__ __forceinline__ void write_tables(const RouteArgs& a, RouteShared& sh, int t0, int tokens) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tiles = tid < a.E ? (sh.total[tid] + kRouteTile - 1) / kRouteTile : 0;
@@ -211,8 +370,14 @@ __device__ __forceinline__ void write_tables(const RouteArgs& a, RouteShared& sh
   }
   if (lane == 31) sh.warp_sum[warp] = inc;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) inc += sh.warp_sum[w];
-  if (tid < a.E) sh.first[tid] = inc - tiles;
+  int up_to = sh.warp_sum[lane];  // of this many warps and the ones before
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, up_to, o);
+    if (lane >= o) up_to += x;
+  }
+  const int used = __shfl_sync(0xffffffffu, up_to, 31), earlier = __shfl_sync(0xffffffffu, up_to, max(warp - 1, 0));
+  if (tid < a.E) sh.first[tid] = inc - tiles + (warp > 0 ? earlier : 0);
   __syncthreads();
   for (int i = tid; i < tokens * a.top_k; i += kRouteThreads) {
     const int tl = i / a.top_k, t = t0 + tl;
@@ -225,45 +390,51 @@ __device__ __forceinline__ void write_tables(const RouteArgs& a, RouteShared& sh
     a.slot_token[slot] = t;
     a.slot_weight[slot] = a.weights[at];
   }
-  // four tiles at a time: their experts and rows, and the slots that hold no token
-  for (int i = blockIdx.x * (kRouteThreads / kRouteTile) + tid / kRouteTile; i < a.n_tiles; i += gridDim.x * (kRouteThreads / kRouteTile)) {
-    int lo = 0, hi = a.E;  // the first expert whose run ends behind tile i
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (sh.first[mid] + (sh.total[mid] + kRouteTile - 1) / kRouteTile > i) hi = mid;
-      else lo = mid + 1;
+  // a warp per expert: the tiles of its run, and the slots behind its last token
+  for (int e = blockIdx.x * (kRouteThreads / 32) + warp; e < a.E; e += gridDim.x * (kRouteThreads / 32)) {
+    const int n = sh.total[e], f = sh.first[e], tl = (n + kRouteTile - 1) / kRouteTile;
+    for (int i = lane; i < tl; i += 32) {
+      a.tile_expert[f + i] = e;
+      a.tile_rows[f + i] = min(n - i * kRouteTile, kRouteTile);
     }
-    const int rows = lo < a.E ? min(sh.total[lo] - (i - sh.first[lo]) * kRouteTile, kRouteTile) : 0;
-    const int r = tid % kRouteTile;
-    if (r == 0) {
-      a.tile_expert[i] = lo < a.E ? lo : -1;
-      a.tile_rows[i] = rows;
+    for (int i = n + lane; i < tl * kRouteTile; i += 32) {
+      a.slot_token[f * kRouteTile + i] = -1;
+      a.slot_weight[f * kRouteTile + i] = 0.f;
     }
-    if (r >= rows) {
-      a.slot_token[i * kRouteTile + r] = -1;
-      a.slot_weight[i * kRouteTile + r] = 0.f;
+  }
+  // the tiles that no run reaches
+  for (int i = used * kRouteTile + blockIdx.x * kRouteThreads + tid; i < a.n_tiles * kRouteTile; i += gridDim.x * kRouteThreads) {
+    a.slot_token[i] = -1;
+    a.slot_weight[i] = 0.f;
+    if (i % kRouteTile == 0) {
+      a.tile_expert[i / kRouteTile] = -1;
+      a.tile_rows[i / kRouteTile] = 0;
     }
   }
 }
 
-template <int P, typename V>
+__device__ __forceinline__ void clear_shared(RouteShared& sh) {
+  for (int e = threadIdx.x; e < kRouteMaxExperts; e += kRouteThreads) sh.mask[e][0] = sh.mask[e][1] = sh.total[e] = sh.before[e] = 0;
+  __syncthreads();
+}
+
+template <int P, bool kScores>
 __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs args) {
   __shared__ RouteShared sh;
-  extern __shared__ double route_scratch[];  // [warp][E] of V where there are groups
+  extern __shared__ double route_scratch[];  // [warp][E] of select_exact (of doubles, whatever it holds), where there are groups
   RouteArgs a = args;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  sh.mask[tid][0] = sh.mask[tid][1] = 0u;
-  __syncthreads();
+  clear_shared(sh);
   grid_dep_wait();
   grid_dep_launch();
   a.logits = after_wait(a.logits);
   a.bias = after_wait(a.bias);
   const int t0 = blockIdx.x * kRouteTokens, tokens = min(a.M - t0, kRouteTokens);
-  V* scratch = reinterpret_cast<V*>(route_scratch) + static_cast<size_t>(warp) * a.E;
+  double* scratch = route_scratch + static_cast<size_t>(warp) * a.E;
   for (int tl = warp; tl < tokens; tl += kRouteThreads / 32) {
     int e;
     float w;
-    choose<P, V>(a, t0 + tl, scratch, e, w);
+    choose<P, kScores>(a, t0 + tl, scratch, e, w);
     if (lane < a.top_k) {
       const size_t at = static_cast<size_t>(t0 + tl) * a.top_k + lane;
       a.experts[at] = e;
@@ -273,59 +444,79 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   }
   if (a.n_tiles == 0) return;
   __syncthreads();
-  const int n = tid < a.E ? __popc(sh.mask[tid][0]) + __popc(sh.mask[tid][1]) : 0;
-  if (gridDim.x > 1) {
-    if (tid < a.E) a.counts[static_cast<size_t>(blockIdx.x) * a.E + tid] = n;
-    return;
+  if (tid < a.E) {
+    const int n = __popc(sh.mask[tid][0]) + __popc(sh.mask[tid][1]);
+    if (gridDim.x > 1) a.counts[static_cast<size_t>(blockIdx.x) * ((a.E + 3) & ~3) + tid] = static_cast<uint8_t>(n);
+    sh.total[tid] = n;
   }
-  sh.total[tid] = n;
-  sh.before[tid] = 0;
-  write_tables(a, sh, t0, tokens);
+  if (gridDim.x == 1) write_tables(a, sh, t0, tokens);
 }
 
 __global__ void __launch_bounds__(kRouteThreads) route_tables_kernel(const RouteArgs args) {
   __shared__ RouteShared sh;
   RouteArgs a = args;
   const int tid = threadIdx.x;
-  sh.mask[tid][0] = sh.mask[tid][1] = 0u;
-  __syncthreads();
+  clear_shared(sh);
   grid_dep_wait();
   grid_dep_launch();
   a.experts = after_wait(a.experts);
   a.weights = after_wait(a.weights);
-  const int* counts = after_wait(a.counts);
   const int t0 = blockIdx.x * kRouteTokens, tokens = min(a.M - t0, kRouteTokens);
   for (int i = tid; i < tokens * a.top_k; i += kRouteThreads) {
     const int tl = i / a.top_k;
     atomicOr(&sh.mask[a.experts[static_cast<size_t>(t0) * a.top_k + i]][tl >> 5], 1u << (tl & 31));
   }
-  int total = 0, before = 0;
-  if (tid < a.E) {
+  // every block adds up the counts of all: four experts to a thread, the blocks shared by the threads
+  const int words = (a.E + 3) / 4, word = tid % words, slices = kRouteThreads / words;
+  const uint32_t* counts = reinterpret_cast<const uint32_t*>(after_wait(a.counts)) + word;
+  if (tid / words < slices) {
+    const int blocks = gridDim.x, self = blockIdx.x;
+    for (int b0 = tid / words; b0 < blocks; b0 += 512 * slices) {  // (512 counts of up to 64 fit 16 bits)
+      uint32_t total[2] = {0u, 0u}, before[2] = {0u, 0u};          // experts 0 and 2, 1 and 3
 #pragma unroll 8
-    for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-      const int n = counts[static_cast<size_t>(b) * a.E + tid];
-      total += n;
-      if (b < static_cast<int>(blockIdx.x)) before += n;
+      for (int b = b0; b < min(blocks, b0 + 512 * slices); b += slices) {
+        const uint32_t n = counts[static_cast<size_t>(b) * words], lo = n & 0x00ff00ffu, hi = n >> 8 & 0x00ff00ffu;
+        total[0] += lo;
+        total[1] += hi;
+        if (b < self) {
+          before[0] += lo;
+          before[1] += hi;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (word * 4 + i < a.E) {  // (integer sums: the same whatever the order)
+          atomicAdd(&sh.total[word * 4 + i], static_cast<int>(total[i & 1] >> (8 * (i & 2)) & 0xffffu));
+          atomicAdd(&sh.before[word * 4 + i], static_cast<int>(before[i & 1] >> (8 * (i & 2)) & 0xffffu));
+        }
     }
   }
-  sh.total[tid] = total;
-  sh.before[tid] = before;
   __syncthreads();
   write_tables(a, sh, t0, tokens);
 }
 
-template <typename V>
-static int32_t launch_choose(const RouteArgs& a, int blocks, size_t smem, cudaStream_t st) {
-  auto go = [&](auto kernel) -> int32_t {
-    if (smem > 32768) QB_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));  // (beside the static tables)
-    return launch_dep("moe_route_scored", kernel, dim3(blocks), dim3(kRouteThreads), smem, st, a);
-  };
+template <int P, bool kScores>
+static int32_t launch_choose(RouteArgs a, int blocks, cudaStream_t st) {
+  const int size = a.E / a.groups, lanes = size / P;
+  a.regular = a.groups == 1 || (size % P == 0 && (lanes & (lanes - 1)) == 0);
+  static std::atomic<unsigned long long> configured{0};  // one bit per device
+  int dev = 0;
+  QB_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || (configured.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+    QB_CUDA_OK(cudaFuncSetAttribute(route_choose_kernel<P, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteThreads / 32 * P * 32 * 8));
+    if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  return launch_dep("moe_route_scored", route_choose_kernel<P, kScores>, dim3(blocks), dim3(kRouteThreads), a.groups > 1 ? static_cast<size_t>(kRouteThreads / 32) * a.E * sizeof(double) : 0, st, a);
+}
+
+template <bool kScores>
+static int32_t launch_choose(const RouteArgs& a, int blocks, cudaStream_t st) {
   const int per_lane = (a.E + 31) / 32;
-  if (per_lane <= 1) return go(route_choose_kernel<1, V>);
-  if (per_lane <= 2) return go(route_choose_kernel<2, V>);
-  if (per_lane <= 4) return go(route_choose_kernel<4, V>);
-  if (per_lane <= 8) return go(route_choose_kernel<8, V>);
-  return go(route_choose_kernel<16, V>);
+  if (per_lane <= 1) return launch_choose<1, kScores>(a, blocks, st);
+  if (per_lane <= 2) return launch_choose<2, kScores>(a, blocks, st);
+  if (per_lane <= 4) return launch_choose<4, kScores>(a, blocks, st);
+  if (per_lane <= 8) return launch_choose<8, kScores>(a, blocks, st);
+  return launch_choose<16, kScores>(a, blocks, st);
 }
 
 static int32_t validate_route(const qb_route_params* p) {
@@ -358,7 +549,7 @@ extern "C" size_t qb_moe_scored_slots(int32_t M, int32_t E, int32_t top_k) {
 
 extern "C" size_t qb_moe_route_scored_workspace_bytes(const qb_route_params* p) {
   if (validate_route(p) != QB_OK || p->M <= kRouteTokens) return 0;
-  return kRouteWsOffset + static_cast<size_t>((p->M + kRouteTokens - 1) / kRouteTokens) * p->E * sizeof(int);
+  return kRouteWsOffset + static_cast<size_t>((p->M + kRouteTokens - 1) / kRouteTokens) * ((p->E + 3) & ~3);
 }
 
 extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, int32_t* experts, float* weights, int32_t* slot_token, float* slot_weight, int32_t* tile_expert,
@@ -383,14 +574,15 @@ extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, in
   a.logits = logits; a.bias = bias; a.f32 = p->logits_dtype == QB_F32; a.sigmoid = p->scoring; a.M = p->M; a.E = p->E; a.top_k = p->top_k;
   a.groups = p->n_groups; a.kept = p->topk_groups; a.top = p->group_top; a.renorm = p->renormalize != 0; a.factor = p->factor;
   if (a.kept == a.groups) a.groups = 1;  // every group is kept
+  a.vec = a.E % (a.f32 ? 4 : 8) == 0;
+  a.vec_bias = aligned16(bias) && a.E % 4 == 0;
   a.experts = experts; a.weights = weights; a.slot_token = slot_token; a.slot_weight = slot_weight; a.tile_expert = tile_expert; a.tile_rows = tile_rows;
   a.token_slot = token_slot;
   a.n_tiles = tables ? static_cast<int>(qb_moe_scored_slots(p->M, p->E, p->top_k) / kRouteTile) : 0;
-  a.counts = tables && blocks > 1 ? reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + kRouteWsOffset) : nullptr;
+  a.counts = tables && blocks > 1 ? static_cast<uint8_t*>(workspace) + kRouteWsOffset : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool wide = bias != nullptr || (a.groups > 1 && a.top == 2);
-  const size_t smem = a.groups > 1 ? static_cast<size_t>(kRouteThreads / 32) * a.E * (wide ? 8 : 4) : 0;
-  rc = wide ? launch_choose<double>(a, blocks, smem, st) : launch_choose<float>(a, blocks, smem, st);
+  const bool scores = bias != nullptr || (a.groups > 1 && a.top == 2);  // (else the choice is the logits')
+  rc = scores ? launch_choose<true>(a, blocks, st) : launch_choose<false>(a, blocks, st);
   if (rc != QB_OK || !tables || blocks == 1) return rc;
   return launch_dep("moe_route_scored (tables)", route_tables_kernel, dim3(blocks), dim3(kRouteThreads), 0, st, a);
 }

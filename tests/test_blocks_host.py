@@ -40,7 +40,7 @@ def test_entry_points_refuse_on_the_host():
         return lib.qb_gemm_blocks(A, B, sa, sb, c, sc, bias, gate, res, C.byref(p), None)
 
     assert gemm(M=0) == -1 and gemm(K=24) == -3 and gemm(N=12) == -3 and gemm(c_dtype=3) == -1 and gemm(activation=2) == -1
-    assert gemm(tile_n=256) == -1 and gemm(split_k=9) == -1 and gemm(A=None) == -1 and gemm(sa=None) == -1 and gemm(sb=None) == -1
+    assert gemm(tile_n=96) == -1 and gemm(split_k=9) == -1 and gemm(A=None) == -1 and gemm(sa=None) == -1 and gemm(sb=None) == -1
     assert gemm(gate=ONE) == -1 and gemm(sc=ONE) == -1 and gemm(c_dtype=1) == -1 and "scales" in last()
     assert gemm(B=C.c_void_p(8)) == -3 and gemm(sb=C.c_void_p(2)) == -3
 
@@ -76,7 +76,7 @@ def test_sizes_of_the_slot_tables():
     p = _lib.RouteParams(M=64, E=256, top_k=8, logits_dtype=2, scoring=1, n_groups=8, topk_groups=4, group_top=2, renormalize=1, factor=1.0)
     assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == 0
     p.M = 129  # behind the area that belongs to the GEMM's tile counters
-    assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == (64 << 10) + 3 * 256 * 4
+    assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == (64 << 10) + 3 * 256
 
 
 @pytest.mark.parametrize("kind,call", [

@@ -229,7 +229,7 @@ def test_epilogues(qb, M, N, K, groups, kind, out):
     check(values(got), scale.to_numpy() if scale else None, y, err, out, f"{M}x{N}x{K} {kind} {out}")
 
 
-@pytest.mark.parametrize("tile_n,split_k", [(64, 1), (128, 1), (64, 2), (64, 4), (64, 8)])
+@pytest.mark.parametrize("tile_n,split_k", [(64, 1), (128, 1), (256, 1), (64, 2), (64, 4), (64, 8)])
 @pytest.mark.parametrize("M,N,K", [(3, 72, 2064), (200, 328, 1040)])
 def test_forced_tiles_and_slices(qb, M, N, K, tile_n, split_k):
     r = util.rng([5, M])
@@ -237,16 +237,20 @@ def test_forced_tiles_and_slices(qb, M, N, K, tile_n, split_k):
     t = op.tensors(qb)
     y, mags = op.product()
     gate, res = bf16_randn(r, (1, N)), bf16_randn(r, (M, N))
+    if split_k == 1 and tile_n > 64:
+        q, s = qb.qf.gemm_blocks(*t, out_dtype="e4m3", tile_n=tile_n)
+        check(values(q), s.to_numpy(), y, op.sum_error(mags), "e4m3", f"{tile_n}")
     for out, kw in (("f32", {}), ("bf16", dict(gate=T(qb, gate, "bf16"), residual=T(qb, res, "bf16"), activation="silu"))):
         got = qb.qf.gemm_blocks(*t, out_dtype=out, tile_n=tile_n, split_k=split_k, b_constant=True, **kw)
         w, err = epilogue(y, op.sum_error(mags), out=out, **(dict(act="silu", gate=gate, residual=res) if kw else {}))
         check(values(got), None, w, err, out, f"{tile_n} {split_k} {out}")
 
 
-def test_power_of_two_result_scales(qb):
+@pytest.mark.parametrize("tile_n", [128, 256])
+def test_power_of_two_result_scales(qb, tile_n):
     r = util.rng(6)
     op = Operands(r, 140, 264, 512)
-    q, s = qb.qf.gemm_blocks(*op.tensors(qb), out_dtype="e4m3", pow2=True)
+    q, s = qb.qf.gemm_blocks(*op.tensors(qb), out_dtype="e4m3", pow2=True, tile_n=tile_n)
     y, mags = op.product()
     err, sc = op.sum_error(mags), s.to_numpy()
     assert np.all(np.frexp(sc)[0] == 0.5)
@@ -291,8 +295,8 @@ def test_quantised_linear_end_to_end(qb):
     ([[33], [5], [128, 64]], 136, 2064),
 ])  # fmt: skip
 @pytest.mark.parametrize("out", ["bf16", "f32", "e4m3"])
-@pytest.mark.parametrize("act", [None, "silu"])
-def test_grouped_product_by_expert_runs(qb, live, N, K, out, act):
+@pytest.mark.parametrize("act,tile_n", [(None, 0), ("silu", 0), (None, 256), ("silu", 128)])
+def test_grouped_product_by_expert_runs(qb, live, N, K, out, act, tile_n):
     r = util.rng([9, N, K])
     table = [(e, n) for e, runs in enumerate(live) for n in runs] + [(-1, 0), (len(live), 128)]  # the last one has no such expert
     te, tr = (np.array(c, np.int32) for c in zip(*table))
@@ -303,7 +307,7 @@ def test_grouped_product_by_expert_runs(qb, live, N, K, out, act):
     o = T(qb, np.full((M, N), 85, carrier), out)
     so = T(qb, np.full((blocks(N), M), -5.0, np.float32)) if out == "e4m3" else None
     before = values(o)[0, 0]
-    qb.qf.gemm_grouped_blocks(A, B, sa, sb, T(qb, te), T(qb, tr), n_experts=E, activation=act, out=o, scale_out=so)
+    qb.qf.gemm_grouped_blocks(A, B, sa, sb, T(qb, te), T(qb, tr), n_experts=E, activation=act, out=o, scale_out=so, tile_n=tile_n)
     got = values(o)
     for i, (e, n) in enumerate(table):
         rows = slice(128 * i, 128 * i + (n if 0 <= e < E else 0))
@@ -319,17 +323,20 @@ def test_grouped_product_by_expert_runs(qb, live, N, K, out, act):
 # --------------------------------------------------------------------------------------------------------------- routing
 
 
-def route(logits, bias, k, scoring, groups=1, kept=1, top=1, renorm=True, factor=1.0):
+def route_scores(logits, scoring):
     x = logits.astype(np.float64)
-    M, E = x.shape
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         if scoring == "softmax":
             m = x.max(1, keepdims=True)
             s = np.exp(x - np.where(np.isinf(m), 0, m))
             t = s.sum(1, keepdims=True)
-            s = np.where(t == 0, 0, s / t)
-        else:
-            s = 1 / (1 + np.exp(-x))
+            return np.where(t == 0, 0, s / t)
+        return 1 / (1 + np.exp(-x))
+
+
+def route(logits, bias, k, scoring, groups=1, kept=1, top=1, renorm=True, factor=1.0):
+    M, E = logits.shape
+    s = route_scores(logits, scoring)
     c = s + (bias.astype(np.float64) if bias is not None else 0)
     if groups > 1 and kept < groups:
         per = -np.sort(-c.reshape(M, groups, -1), 2)[:, :, :top].sum(2)
@@ -424,6 +431,47 @@ def test_routing_of_equal_and_masked_logits(qb, scoring, groups, kept, top, bias
     else:
         check_routing(got, got.experts.to_numpy(), w, E)  # (which of several experts of score 0 is left open)
     assert np.all(got.weights.to_numpy()[5] == 0)
+
+
+@pytest.mark.parametrize("E,k,groups,kept,top", [(64, 6, 1, 1, 1), (64, 6, 8, 3, 2), (256, 32, 1, 1, 1), (16, 15, 1, 1, 1), (16, 16, 1, 1, 1), (40, 3, 8, 2, 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dense", [False, True])
+def test_routing_of_close_scores(qb, E, k, groups, kept, top, scoring, dense):
+    """Scores that differ by less than a rounding to 32 bits are told apart, be it two of them or all."""
+    r = util.rng([15, E, k])
+    M = 200
+    x = (1.5 * r.standard_normal((M, E))).astype(np.float32)
+    bias = (0.1 * r.standard_normal(E)).astype(np.float32)
+    if dense:
+        x = (np.float32(0.5) + r.integers(-4, 5, (M, E)).astype(np.float32) * np.float32(2.0**-24)).astype(np.float32)
+        bias[:] = r.integers(0, 2, E) * np.float32(0.25)
+    else:  # expert 1 scores as expert 0 to the last bit or so, and expert 2 as 3 in other tokens
+        for m in range(M):
+            p, q = (0, 1) if m % 2 else (3, 2)
+            s = 1 / (1 + np.exp(-x[m].astype(np.float64)))
+            want = s[p] + float(bias[p]) - float(bias[q])
+            if 1e-3 < want < 1 - 1e-3:
+                x[m, q] = np.float32(np.log(want / (1 - want)))
+                x[m, [p, q]] += np.float32(2.0) if m % 3 == 0 else 0
+    got = qb.qf.moe_route_scored(T(qb, x), T(qb, bias), top_k=k, scoring=scoring, n_groups=groups, topk_groups=kept, group_top=top)
+    e, w = route(x, bias, k, scoring, groups, kept, top)
+    if dense and groups > 1:
+        # Two experts one step up and down sum to two in the middle but for (2^-24)^2 of a score: below 2^-50, so 64 bits do not say which
+        # group is first.  Any of the groups that close to the last one kept will do; the choice inside them is the formula's.
+        c = route_scores(x, scoring) + bias.astype(np.float64)
+        per = -np.sort(-c.reshape(M, groups, -1), 2)[:, :, :top].sum(2)
+        last = -np.sort(-per, 1)[:, kept - 1]
+        ge = got.experts.to_numpy()
+        for m in range(M):
+            used = set(ge[m] // (E // groups))
+            assert all(per[m, g] >= last[m] - 2.0**-50 for g in used)
+            kept_now = used | {g for g in range(groups) if per[m, g] > last[m] + 2.0**-50}
+            assert len(kept_now) <= kept
+            inside = np.where(np.isin(np.arange(E) // (E // groups), list(kept_now)), c[m], -np.inf)
+            np.testing.assert_array_equal(ge[m], np.argsort(-inside, kind="stable")[:k])
+        s = np.take_along_axis(route_scores(x, scoring), ge, 1)
+        e, w = ge, s / s.sum(1, keepdims=True)
+    check_routing(got, e, w, E)
 
 
 def test_routing_of_nan(qb):
