@@ -14,7 +14,8 @@
 //     with 16 warps of half the columns (what every warp does once a block filled the schedulers), and take 330 (64 columns) and 420 (128).
 // 24.5 -> 16.4 us and 28.3 -> 18.6 us at that size.
 //
-// Warp 0 TMA, warp 1 MMA, warps 2-9 sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
+// A CTA stays for all tiles of its share: while its warps are in the epilogue of one, the copies and the MMAs of the next go on.
+// Warp 0 TMA, warp 1 MMA, warps 2-9 (4-11 with 256 columns) sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
 #include <atomic>
 
 #include "gemm_common.cuh"
@@ -102,30 +103,46 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   float* tops = reinterpret_cast<float*>(smem + L::kTopOffset);  // 128 columns: [column group][row], largest magnitude of a thread's columns
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * BN, m0 = blockIdx.y * kBM, split = blockIdx.z;
+  const int split = blockIdx.z;
   const int kb0 = split * g.kb_per_split, n_iter = min(kb0 + g.kb_per_split, g.kb_total) - kb0;
-  const bool clustered = BN == 64 && g.cluster != 0;
-  int expert = 0, rows = min(g.M - m0, kBM);
+  const bool clustered = BN == 64 && g.cluster != 0;  // one tile per cluster
   if (GROUPED) {
     grid_dep_wait();  // the tables are written by the routing kernel
     grid_dep_launch();
-    expert = after_wait(g.tile_expert)[blockIdx.y];
-    if (expert < 0 || expert >= args.n_experts) return;  // a padding tile
-    rows = min(max(after_wait(args.tile_rows)[blockIdx.y], 0), kBM);
-    if (rows == 0) return;
   }
-  const bool small = GROUPED && rows <= args.small_rows;
-  const int a_rows = small ? args.small_rows : g.a_rows;
-  const uint32_t stage_tx = a_rows * kRowBytes + BN * kRowBytes;
+  // Where tile t of the walk lies; false for one without tokens.  Dense: groups of 8 row tiles, the row index fastest, so that what runs at the
+  // same time shares row tiles of A and column tiles of B.  Grouped: the columns of a row tile together.
+  const int tiles_n = g.n_tiles / g.tiles_m;
+  auto locate = [&](int t, int& m0, int& n0, int& rows, int& expert) {
+    int mt, nt;
+    if (GROUPED) {
+      mt = t / tiles_n;
+      nt = t - mt * tiles_n;
+    } else {
+      const int group = t / (8 * tiles_n), gm = min(g.tiles_m - 8 * group, 8), i = t - group * 8 * tiles_n;
+      nt = i / gm;
+      mt = 8 * group + i - nt * gm;
+    }
+    m0 = mt * kBM;
+    n0 = nt * BN;
+    expert = 0;
+    rows = min(g.M - m0, kBM);
+    if (GROUPED) {
+      expert = after_wait(g.tile_expert)[mt];
+      rows = min(after_wait(args.tile_rows)[mt], kBM);
+      return expert >= 0 && expert < args.n_experts && rows > 0;
+    }
+    return true;
+  };
 
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(small ? &tmA_small : &tmA);
+    tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
-    for (int b = 0; b < kAccBuffers; ++b) mbar_init(smem_u32(&acc_empty[b]), kColGroups * ((rows + 31) / 32));  // of the warps that have a row
+    for (int b = 0; b < kAccBuffers; ++b) mbar_init(smem_u32(&acc_empty[b]), kSumWarps);
     *abort_flag = 0;
     *drain_flag = 0;
     *lost_flag = 0;
@@ -146,36 +163,53 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   if (warp == 0) {
     // ---------------- TMA producer
     if (elect_one()) {
-      const CUtensorMap* a_map = small ? &tmA_small : &tmA;
-      const int b_row0 = expert * g.N + n0;
       const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), stage0 = smem_u32(smem);
-      // constant weights do not depend on the kernels before this one: their first tiles are on the way while those finish
-      const int ahead = !GROUPED && g.b_const ? min(kStages, n_iter) : 0;
-      for (int it = 0; it < ahead; ++it) {
-        mbar_arrive_expect_tx(full0 + it * 8, stage_tx);
-        tma_load_2d(stage0 + it * L::kStageBytes + kBM * kRowBytes, &tmB, full0 + it * 8, (kb0 + it) * 128, b_row0);
-      }
-      if (!GROUPED) grid_dep_wait();
-      for (int it = 0; it < ahead; ++it) tma_load_2d(stage0 + it * L::kStageBytes, a_map, full0 + it * 8, (kb0 + it) * 128, m0);
-      int it = ahead, s = ahead == kStages ? 0 : ahead;
-      uint32_t ph = ahead == kStages ? 0 : 1;  // (a fresh barrier passes for parity 1)
+      int s = 0;
+      uint32_t ph = 1;  // (a fresh barrier passes for parity 1)
+      bool alive = true, waited = GROUPED;
+      for (int t = blockIdx.x; t < g.n_tiles && alive; t += gridDim.x) {
+        int m0, n0, rows, expert;
+        if (!locate(t, m0, n0, rows, expert)) continue;
+        const bool small = GROUPED && rows <= args.small_rows;
+        const CUtensorMap* a_map = small ? &tmA_small : &tmA;
+        const uint32_t stage_tx = (small ? args.small_rows : g.a_rows) * kRowBytes + BN * kRowBytes;
+        const int b_row0 = expert * g.N + n0;
+        int it = 0;
+        if (!waited) {
+          // constant weights do not depend on the kernels before this one: their first tiles are on the way while those finish
+          const int ahead = g.b_const ? min(kStages, n_iter) : 0;
+          for (; it < ahead; ++it) {
+            mbar_arrive_expect_tx(full0 + it * 8, stage_tx);
+            tma_load_2d(stage0 + it * L::kStageBytes + kBM * kRowBytes, &tmB, full0 + it * 8, (kb0 + it) * 128, b_row0);
+          }
+          grid_dep_wait();
+          for (int i = 0; i < ahead; ++i) tma_load_2d(stage0 + i * L::kStageBytes, a_map, full0 + i * 8, (kb0 + i) * 128, m0);
+          waited = true;
+          s = ahead == kStages ? 0 : ahead;
+          ph = ahead == kStages ? 0 : 1;
+        }
 #pragma unroll 2
-      for (; it < n_iter; ++it) {
-        if (!mbar_wait(empty0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        const uint32_t fb = full0 + s * 8, st = stage0 + s * L::kStageBytes;
-        mbar_arrive_expect_tx(fb, stage_tx);
-        tma_load_2d(st + kBM * kRowBytes, &tmB, fb, (kb0 + it) * 128, b_row0);
-        tma_load_2d(st, a_map, fb, (kb0 + it) * 128, m0);
-        if (++s == kStages) { s = 0; ph ^= 1; }
+        for (; it < n_iter; ++it) {
+          alive = mbar_wait(empty0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+          if (!alive) break;
+          const uint32_t fb = full0 + s * 8, st = stage0 + s * L::kStageBytes;
+          mbar_arrive_expect_tx(fb, stage_tx);
+          tma_load_2d(st + kBM * kRowBytes, &tmB, fb, (kb0 + it) * 128, b_row0);
+          tma_load_2d(st, a_map, fb, (kb0 + it) * 128, m0);
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
+      }
+      if (alive && *abort_flag == 0) {
+        // Tail: see the last stage releases land before the CTA can exit (a stage that was never used passes at once).
+        for (int i = 0; i < kStages; ++i) {
+          if (!mbar_wait(empty0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
       }
       if (*abort_flag) {
-        // Giving up: let the copies already in flight land before this CTA's memory goes away.
-        for (int i = max(0, it - kStages); i < it; ++i)
-          mbar_wait(full0 + i % kStages * 8, (i / kStages) & 1, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
-      } else {
-        // Tail: see the last stage releases land before the CTA can exit.
-        for (int i = max(0, n_iter - kStages); i < n_iter; ++i)
-          if (!mbar_wait(empty0 + i % kStages * 8, (i / kStages) & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+        // Giving up: leave the copies already in flight time to land before this CTA's memory goes away.
+        const long long t0 = clock64();
+        while (clock64() - t0 < (1ll << 22)) __nanosleep(1000);
       }
     }
   } else if (warp == 1) {
@@ -183,75 +217,76 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if (elect_one()) {
       const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), taken0 = smem_u32(acc_empty);
       const uint64_t desc0 = umma_desc_k_sw128(smem_u32(smem));
-      int s = 0, buf = 0;
-      uint32_t ph = 0, bph = 1;  // (a fresh buffer passes for parity 1)
-      bool landed = false, taken = true;  // what the barriers of this stage and buffer said a block earlier
-#pragma unroll 4
-      for (int it = 0; it < n_iter; ++it) {
-        if (!landed && !mbar_wait(full0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        if (!taken && !mbar_wait(taken0 + buf * 8, bph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        tc_fence_after();
-        const uint64_t a_desc = desc0 + static_cast<uint64_t>(s * (L::kStageBytes >> 4)), b_desc = a_desc + (kBM * kRowBytes >> 4);
-        const uint32_t d = tmem_base + buf * BN, release = empty0 + s * 8;
-        if (++s == kStages) { s = 0; ph ^= 1; }
-        if (++buf == kAccBuffers) { buf = 0; bph ^= 1; }
-        landed = mbar_test_wait(full0 + s * 8, ph);
-        taken = mbar_test_wait(taken0 + buf * 8, bph);
+      int s = 0;
+      uint32_t ph = 0, bph = ~0u;  // bit b: parity to wait for at buffer b (a fresh one passes for parity 1); a tile begins with buffer 0
+      bool landed = false, taken = false;  // what the barriers of this stage and buffer said a block earlier
+      bool alive = true;
+      for (int t = blockIdx.x; t < g.n_tiles && alive; t += gridDim.x) {
+        int m0, n0, rows, expert;
+        if (!locate(t, m0, n0, rows, expert)) continue;
+#pragma unroll 1
+        for (int base = 0; base < n_iter && alive; base += 4) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f8(d, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k > 0 ? 1u : 0u);
-        if (it == n_iter - 1 && late(blockIdx.x == gridDim.x - 1 && blockIdx.z == gridDim.z - 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-        umma_commit(release);  // (not reached: the other warps give up as well)
+          for (int i = 0; i < 4; ++i) {
+            const int it = base + i;
+            if (it >= n_iter) break;
+            constexpr uint32_t kOne = 1;
+            const int buf = i % kAccBuffers, after = (i + 1) % kAccBuffers;
+            alive = (landed || mbar_wait(full0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) &&
+                    (taken || mbar_wait(taken0 + buf * 8, bph >> buf & 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM));
+            if (!alive) break;
+            tc_fence_after();
+            const uint64_t a_desc = desc0 + static_cast<uint64_t>(s * (L::kStageBytes >> 4)), b_desc = a_desc + (kBM * kRowBytes >> 4);
+            const uint32_t release = empty0 + s * 8;
+            if (++s == kStages) { s = 0; ph ^= 1; }
+            bph ^= kOne << buf;
+            landed = mbar_test_wait(full0 + s * 8, ph);
+            taken = it + 1 < n_iter && mbar_test_wait(taken0 + after * 8, bph >> after & 1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) umma_f8(tmem_base + buf * BN, a_desc + 2 * k, b_desc + 2 * k, kIdesc, k > 0 ? 1u : 0u);
+            if (it == n_iter - 1 && late(t + static_cast<int>(gridDim.x) >= g.n_tiles && blockIdx.x == gridDim.x - 1 && blockIdx.z == gridDim.z - 1, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) {
+              alive = false;  // (the products are never announced: the other warps give up as well)
+              break;
+            }
+            umma_commit(release);
+          }
+        }
       }
     }
   } else if (warp >= kW0) {
     // ---------------- sums and epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31
     if (BN == 256) setmaxnreg_inc<kWideSumRegs>();
     const int lane_grp = warp & 3, group = (warp - kW0) >> 2, et = threadIdx.x - 32 * kW0;
-    const int row = lane_grp * 32 + lane, m = m0 + row;
-    const bool live = row < rows, busy = lane_grp * 32 < rows;  // this thread's row, any row of this warp
+    const int row = lane_grp * 32 + lane;
     if (!GROUPED) grid_dep_wait();
-    const int m_last = m0 + rows - 1;
-    const bool one_gate = g.gate == nullptr || m0 / g.rows_per_gate == m_last / g.rows_per_gate;
     const int slice_rows = kBM / (clustered ? g.splits : 1), slice_row0 = clustered ? split * slice_rows : 0;  // rows this CTA finishes
-    // The scales of this thread's row and of its columns, loaded kScales blocks ahead: behind the operands' traffic a load takes over
-    // 1000 clocks, as long as four blocks of 64 columns.  (Rows and blocks past the last are read as the last, without a branch.)
-    const int nb = (g.N + 127) / 128;  // (256 columns: a thread's 128 are one block's)
-    const float* as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + min(m, m_last);
-    const float* bs = after_wait(args.b_scale) + static_cast<size_t>(expert * nb + min(n0 / 128 + (BN == 256 ? group : 0), nb - 1)) * g.kb_total + kb0;
+    const int nb = (g.N + 127) / 128;
+    int m0 = 0, n0 = 0, rows = 0;
+    // The scales of this thread's row and of its columns (of 256 columns, a thread's 128 are one block's), loaded kScales blocks ahead:
+    // behind the operands' traffic a load takes over 1000 clocks, as long as four blocks of 64 columns.  (Rows and blocks past the last
+    // are read as the last, without a branch.)
+    const float *as = nullptr, *bs = nullptr;
     float sa[kScales], sb[kScales];
     auto fetch_scales = [&](int j, int it) {
       const unsigned at = min(it, n_iter - 1);
       sa[j] = as[static_cast<size_t>(at) * static_cast<unsigned>(g.M)];
       sb[j] = bs[at];
     };
+    // the first tile from t on that has tokens, with its first scales on their way; n_tiles behind the last
+    auto tile_from = [&](int t) {
+      for (; t < g.n_tiles; t += gridDim.x) {
+        int expert;
+        if (!locate(t, m0, n0, rows, expert)) continue;
+        as = after_wait(args.a_scale) + static_cast<size_t>(kb0) * g.M + min(m0 + row, m0 + rows - 1);
+        bs = after_wait(args.b_scale) + static_cast<size_t>(expert * nb + min(n0 / 128 + (BN == 256 ? group : 0), nb - 1)) * g.kb_total + kb0;
 #pragma unroll
-    for (int j = 0; j < kScales; ++j) fetch_scales(j, j);
-    // the tile's per-column vectors, and the residuals of the 8-column groups that this thread finishes for the cluster
-    for (int j = et; j < BN; j += kSumThreads) {
-      const int n = n0 + j;
-      const bool in = n < g.N;
-      col[BN + j] = (in && g.bias) ? bf16_bits_to_f32(g.bias[n]) : 0.f;
-      col[2 * BN + j] = (in && g.gate) ? bf16_bits_to_f32(g.gate[static_cast<size_t>(m0 / g.rows_per_gate) * g.N + n]) : 0.f;
-    }
-    uint4 pre[BN / 32][2];
-    if (clustered && one_gate && g.gate != nullptr && et < 256) {
-#pragma unroll
-      for (int k = 0; k < BN / 32; ++k) {
-        const int r = et / (BN / 8) + 256 / (BN / 8) * k, mm = m0 + slice_row0 + r, n = n0 + et % (BN / 8) * 8;
-        pre[k][0] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < slice_rows && mm < g.M && n < g.N) pre[k][0] = *reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(mm) * g.N + n);
+        for (int j = 0; j < kScales; ++j) fetch_scales(j, j);
+        break;
       }
-    }
-    asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
-
-    const uint32_t taddr = tmem_base + (static_cast<uint32_t>(lane_grp * 32) << 16) + group * kCols;
-    float2 acc[kCols / 2];
-#pragma unroll
-    for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
-    // Of a thread's columns one part is on its way from TMEM while the last one is added.
-    constexpr int kPart = kCols / 2 < 32 ? kCols / 2 : 32, kParts = kCols / kPart;
-    uint32_t t[2][kPart];
-    const uint32_t done0 = smem_u32(empty_bar);
+      return t;
+    };
+    const uint32_t tbase = tmem_base + (static_cast<uint32_t>(lane_grp * 32) << 16) + group * kCols;
+    const uint32_t done0 = smem_u32(empty_bar), taken0 = smem_u32(acc_empty);
     int ws = 0;
     uint32_t wph = 0;
     auto next_block = [&]() {
@@ -259,152 +294,239 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       if (++ws == kStages) { ws = 0; wph ^= 1; }
       tc_fence_after();
     };
-    if (busy) {
-      next_block();
-      tmem_ld(taddr, t[0]);
-#pragma unroll 1
-      for (int base = 0; base < n_iter; base += kScales) {
+    auto release = [&](int buf) {  // its products have been read
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(taken0 + buf * 8);
+    };
+    for (int tile = tile_from(blockIdx.x), next; tile < g.n_tiles; tile = next) {
+      const int m = m0 + row, m_last = m0 + rows - 1, n0_of = n0;
+      const bool live = row < rows, busy = lane_grp * 32 < rows;  // this thread's row, any row of this warp
+      const bool one_gate = g.gate == nullptr || m0 / g.rows_per_gate == m_last / g.rows_per_gate;
+      // the tile's per-column vectors, and the residuals of the 8-column groups that this thread finishes for the cluster
+      if (g.bias != nullptr || g.gate != nullptr) {
+        asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");  // the last tile's readers are done
+        for (int j = et; j < BN; j += kSumThreads) {
+          const int n = n0 + j;
+          const bool in = n < g.N;
+          col[BN + j] = (in && g.bias) ? bf16_bits_to_f32(g.bias[n]) : 0.f;
+          col[2 * BN + j] = (in && g.gate) ? bf16_bits_to_f32(g.gate[static_cast<size_t>(m0 / g.rows_per_gate) * g.N + n]) : 0.f;
+        }
+      }
+      uint4 pre[BN == 64 ? BN / 32 : 1][2];
+      if constexpr (BN == 64) {
+        if (clustered && one_gate && g.gate != nullptr) {
 #pragma unroll
-        for (int j = 0; j < kScales; ++j) {
-          const int it = base + j;
-          if (it >= n_iter) break;
-          const uint32_t from = taddr + j % kAccBuffers * BN;
-          const float s = sa[j] * sb[j];
-          const float2 s2 = make_float2(s, s);
-          fetch_scales(j, it + kScales);
+          for (int k = 0; k < BN / 32; ++k) {
+            const int r = et / (BN / 8) + 256 / (BN / 8) * k, mm = m0 + slice_row0 + r, n = n0 + et % (BN / 8) * 8;
+            pre[k][0] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < slice_rows && mm < g.M && n < g.N) pre[k][0] = *reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(mm) * g.N + n);
+          }
+        }
+      }
+      float2 acc[kCols / 2];
+#pragma unroll
+      for (int j = 0; j < kCols / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+      // Of a thread's columns one part is on its way from TMEM while the last one is added.  The last block's buffer is kept: the
+      // sums go back there for the epilogue, while the MMAs of the next tile fill the others.
+      constexpr int kPart = kCols / 2 < 32 ? kCols / 2 : 32, kParts = kCols / kPart;
+      uint32_t t[2][kPart];
+      next_block();
+      if (busy) {
+        tmem_ld(tbase, t[0]);
+#pragma unroll 1
+        for (int base = 0; base < n_iter; base += kScales) {
+#pragma unroll
+          for (int j = 0; j < kScales; ++j) {
+            const int it = base + j;
+            if (it >= n_iter) break;
+            const uint32_t from = tbase + j % kAccBuffers * BN;
+            const float s = sa[j] * sb[j];
+            const float2 s2 = make_float2(s, s);
+            fetch_scales(j, it + kScales);
+#pragma unroll
+            for (int c = 0; c < kParts; ++c) {
+              tmem_wait_ld_into(t[c & 1]);
+              if (c + 1 < kParts) {
+                tmem_ld(from + (c + 1) * kPart, t[(c + 1) & 1]);
+              } else if (it + 1 < n_iter) {
+                release(j % kAccBuffers);
+                next_block();
+                tmem_ld(tbase + (j + 1) % kAccBuffers * BN, t[0]);
+              }
+#pragma unroll
+              for (int q = 0; q < kPart / 2; ++q) fma2(acc[c * (kPart / 2) + q], __uint_as_float(t[c & 1][2 * q]), __uint_as_float(t[c & 1][2 * q + 1]), s2);
+            }
+          }
+        }
+      } else {
+        for (int it = 1; it < n_iter; ++it) {
+          release((it - 1) % kAccBuffers);
+          next_block();
+        }
+      }
+      const int last_buf = (n_iter - 1) % kAccBuffers;
+      const uint32_t taddr = tbase + last_buf * BN;
+      bool ok = all_of_epilogue<kSumThreads>(*abort_flag == 0);  // (and the column vectors are in place)
+      next = tile_from(tile + gridDim.x);  // m0, n0 and rows are the next tile's from here on
+      const bool precise = g.c_dtype != QB_BF16;
+      if (clustered) {
+        if constexpr (BN == 64) {
+          if (ok) {
+            const uint32_t dst = map_to_cta(smem_u32(smem + L::kSliceOffset), row / slice_rows);
+#pragma unroll
+            for (int v = 0; v < kCols / 4; ++v)
+              st_dsmem_v4(dst + 16 * slice_unit<BN>(split, group * (kCols / 4) + v, row % slice_rows, slice_rows), __float_as_uint(acc[2 * v].x), __float_as_uint(acc[2 * v].y),
+                          __float_as_uint(acc[2 * v + 1].x), __float_as_uint(acc[2 * v + 1].y));
+          } else if (threadIdx.x == 64) {
+            tell_lost<1>(lost_flag, 0, g.splits);
+          }
+          cluster_sync();  // every slice's share of this CTA's rows has arrived after this barrier (warps 0 and 1 join it below)
+          if (ok && *lost_flag == 0) {
+            const float4* parts = reinterpret_cast<const float4*>(smem + L::kSliceOffset);
+            if (precise) finish_slices<BN, true>(g, parts, col, m - row, n0_of, slice_row0, slice_rows, one_gate, pre);
+            else finish_slices<BN, false>(g, parts, col, m - row, n0_of, slice_row0, slice_rows, one_gate, pre);
+          }
+        }
+      } else {
+        const bool narrow = args.c_scale != nullptr;
+        if (BN == 128 && narrow) {
+          // A row's group of 128 results lies with two threads: values in the registers of the sums, the larger of their maxima through
+          // shared memory.  (Through TMEM and 16 columns at a time, two passes of a loop, a tile took 1.8 us longer.)
+          if constexpr (BN == 128) {
+            float top = 0.f;
+            if (ok && live) {
+#pragma unroll
+              for (int c = 0; c < kCols; c += 16) {
+                const int n = n0_of + group * kCols + c;
+                if (n < g.N) {
+                  float v[16];
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) {
+                    v[2 * q] = acc[c / 2 + q].x;
+                    v[2 * q + 1] = acc[c / 2 + q].y;
+                  }
+                  epilogue16_values<BN, true>(g, v, m, n, col + group * kCols + c, reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(m) * g.N + n), one_gate);
+#pragma unroll
+                  for (int q = 0; q < 8; ++q) {
+                    if (q < 4 || n + 8 < g.N) top = fmaxf(top, fmaxf(fabsf(v[2 * q]), fabsf(v[2 * q + 1])));
+                    acc[c / 2 + q] = make_float2(v[2 * q], v[2 * q + 1]);
+                  }
+                }
+              }
+            }
+            tops[group * kBM + row] = top;
+            asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
+            if (ok && live) {
+              const float s = block_scale(fmaxf(tops[row], tops[kBM + row]), args.pow2 != 0), inv = __frcp_rn(s);
+              if (group == 0) args.c_scale[static_cast<size_t>(n0_of / 128) * g.M + m] = s;
+              uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
+#pragma unroll
+              for (int c = 0; c < kCols; c += 16) {
+                const int n = n0_of + group * kCols + c;
+                uint32_t w[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const float2 x = acc[c / 2 + 2 * q], y = acc[c / 2 + 2 * q + 1];
+                  w[q] = pack_e4m3x4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(y.x, inv), __fmul_rn(y.y, inv));
+                }
+                if (n >= g.N) continue;
+                if (g.N % 16 == 0) {
+                  *reinterpret_cast<uint4*>(c_row + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                  *reinterpret_cast<uint2*>(c_row + n) = make_uint2(w[0], w[1]);
+                  if (n + 8 < g.N) *reinterpret_cast<uint2*>(c_row + n + 8) = make_uint2(w[2], w[3]);
+                }
+              }
+            }
+          }
+        } else if (ok && busy) {
+          float row_top = 0.f;
+          // (a warp reads back what it wrote itself)
 #pragma unroll
           for (int c = 0; c < kParts; ++c) {
-            tmem_wait_ld_into(t[c & 1]);
-            if (c + 1 < kParts) {
-              tmem_ld(from + (c + 1) * kPart, t[(c + 1) & 1]);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&acc_empty[j % kAccBuffers]));
-              if (it + 1 < n_iter) {
-                next_block();
-                tmem_ld(taddr + (j + 1) % kAccBuffers * BN, t[0]);
-              }
+#pragma unroll
+            for (int q = 0; q < kPart / 2; ++q) {
+              t[c & 1][2 * q] = __float_as_uint(acc[c * (kPart / 2) + q].x);
+              t[c & 1][2 * q + 1] = __float_as_uint(acc[c * (kPart / 2) + q].y);
             }
-#pragma unroll
-            for (int q = 0; q < kPart / 2; ++q) fma2(acc[c * (kPart / 2) + q], __uint_as_float(t[c & 1][2 * q]), __uint_as_float(t[c & 1][2 * q + 1]), s2);
+            tmem_st(taddr + c * kPart, t[c & 1]);
           }
-        }
-      }
-    }
-    bool ok = *abort_flag == 0;
-    const bool precise = g.c_dtype != QB_BF16;
-    if (clustered) {
-      if constexpr (BN == 64) {
-        ok = all_of_epilogue<kSumThreads>(ok);
-        if (ok) {
-          const uint32_t dst = map_to_cta(smem_u32(smem + L::kSliceOffset), row / slice_rows);
-#pragma unroll
-          for (int v = 0; v < kCols / 4; ++v)
-            st_dsmem_v4(dst + 16 * slice_unit<BN>(split, group * (kCols / 4) + v, row % slice_rows, slice_rows), __float_as_uint(acc[2 * v].x), __float_as_uint(acc[2 * v].y),
-                        __float_as_uint(acc[2 * v + 1].x), __float_as_uint(acc[2 * v + 1].y));
-        } else if (threadIdx.x == 64) {
-          tell_lost<1>(lost_flag, 0, g.splits);
-        }
-        cluster_sync();  // every slice's share of this CTA's rows has arrived after this barrier (warps 0 and 1 join it below)
-        if (ok && *lost_flag == 0 && et < 256) {
-          const float4* parts = reinterpret_cast<const float4*>(smem + L::kSliceOffset);
-          if (precise) finish_slices<BN, true>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
-          else finish_slices<BN, false>(g, parts, col, m0, n0, slice_row0, slice_rows, one_gate, pre);
-        }
-      }
-    } else {
-      const bool narrow = args.c_scale != nullptr;
-      float row_top = 0.f;
-      if (BN == 128 && narrow) ok = all_of_epilogue<kSumThreads>(ok);  // the two threads of a row's 128 columns meet at a barrier
-      if (ok && busy) {
-        // every MMA of the CTA is done (this warp has waited for each block), and a warp reads back what it wrote itself
-#pragma unroll
-        for (int c = 0; c < kParts; ++c) {
-#pragma unroll
-          for (int q = 0; q < kPart / 2; ++q) {
-            t[c & 1][2 * q] = __float_as_uint(acc[c * (kPart / 2) + q].x);
-            t[c & 1][2 * q + 1] = __float_as_uint(acc[c * (kPart / 2) + q].y);
-          }
-          tmem_st(taddr + c * kPart, t[c & 1]);
-        }
-        tmem_wait_st();
-        const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.C) & 31u) == 0;
-        uint8_t* c_row = live ? row_of_c(g, m) : nullptr;
-        const uint4* res_row = reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(m) * g.N + n0);
-        const int c0 = group * kCols;
-        uint4 next[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};  // residual of the next turn
-        auto fetch = [&](int c) {
-          if (g.gate != nullptr && c < c0 + kCols && live && n0 + c < g.N) {
-            next[0] = res_row[c / 8];
-            if (n0 + c + 8 < g.N) next[1] = res_row[c / 8 + 1];
-          }
-        };
-        fetch(c0);
-        float top = 0.f;
-#pragma unroll 1
-        for (int c = c0; c < c0 + kCols; c += 16) {
-          if (n0 + c >= g.N) break;
-          uint4 res[2] = {next[0], next[1]};
-          uint32_t r[16];
-          tmem_ld16(taddr + c - c0, r);
-          fetch(c + 16);
-          tmem_wait_ld_into(r);
-          if (!narrow) {
-            if (!live) continue;
-            if (precise) epilogue16<BN, true>(g, r, m, n0 + c, col + c, res, one_gate, c_row, wide, true);
-            else epilogue16<BN, false>(g, r, m, n0 + c, col + c, res, one_gate, c_row, wide, true);
-          } else {
-            float v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-            if (live) epilogue16_values<BN, true>(g, v, m, n0 + c, col + c, res, one_gate);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (j < 8 || n0 + c + 8 < g.N) top = fmaxf(top, fabsf(v[j]));
-              r[j] = __float_as_uint(v[j]);
-            }
-            tmem_st16(taddr + c - c0, r);
-          }
-        }
-        if (narrow) {
           tmem_wait_st();
-          if (BN == 128) tops[group * kBM + row] = top;
-          row_top = top;
-        }
-      }
-      if constexpr (BN >= 128) {
-        if (narrow && ok) {
-          if (BN == 128) asm volatile("bar.sync 2, %0;" ::"n"(kSumThreads) : "memory");
-          if (busy) {
-            if (BN == 128) row_top = fmaxf(tops[row], tops[kBM + row]);
-            const float s = block_scale(row_top, args.pow2 != 0), inv = __frcp_rn(s);
-            const int block = n0 / 128 + (BN == 256 ? group : 0);
-            if (live && (BN == 256 ? block < nb : group == 0)) args.c_scale[static_cast<size_t>(block) * g.M + m] = s;
-            uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
-            const bool wide = g.N % 16 == 0;
+          const bool wide = g.N % 32 == 0 && (reinterpret_cast<uintptr_t>(g.C) & 31u) == 0;
+          uint8_t* c_row = live ? row_of_c(g, m) : nullptr;
+          const uint4* res_row = reinterpret_cast<const uint4*>(g.residual + static_cast<size_t>(m) * g.N + n0_of);
+          const int c0 = group * kCols;
+          uint4 coming[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};  // residual of the next turn
+          auto fetch = [&](int c) {
+            if (g.gate != nullptr && c < c0 + kCols && live && n0_of + c < g.N) {
+              coming[0] = res_row[c / 8];
+              if (n0_of + c + 8 < g.N) coming[1] = res_row[c / 8 + 1];
+            }
+          };
+          fetch(c0);
+          float top = 0.f;
 #pragma unroll 1
-            for (int c = group * kCols; c < (group + 1) * kCols; c += 16) {
-              const int n = n0 + c;
-              if (n >= g.N) break;
-              uint32_t r[16], w[4];
-              tmem_ld16(taddr + c - group * kCols, r);
-              tmem_wait_ld_into(r);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w[j] = pack_e4m3x4(__fmul_rn(__uint_as_float(r[4 * j]), inv), __fmul_rn(__uint_as_float(r[4 * j + 1]), inv), __fmul_rn(__uint_as_float(r[4 * j + 2]), inv),
-                                   __fmul_rn(__uint_as_float(r[4 * j + 3]), inv));
+          for (int c = c0; c < c0 + kCols; c += 16) {
+            if (n0_of + c >= g.N) break;
+            uint4 res[2] = {coming[0], coming[1]};
+            uint32_t r[16];
+            tmem_ld16(taddr + c - c0, r);
+            fetch(c + 16);
+            tmem_wait_ld_into(r);
+            if (!narrow) {
               if (!live) continue;
-              if (wide) {
-                *reinterpret_cast<uint4*>(c_row + n) = make_uint4(w[0], w[1], w[2], w[3]);
-              } else {
-                *reinterpret_cast<uint2*>(c_row + n) = make_uint2(w[0], w[1]);
-                if (n + 8 < g.N) *reinterpret_cast<uint2*>(c_row + n + 8) = make_uint2(w[2], w[3]);
+              if (precise) epilogue16<BN, true>(g, r, m, n0_of + c, col + c, res, one_gate, c_row, wide, true);
+              else epilogue16<BN, false>(g, r, m, n0_of + c, col + c, res, one_gate, c_row, wide, true);
+            } else {
+              float v[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+              if (live) epilogue16_values<BN, true>(g, v, m, n0_of + c, col + c, res, one_gate);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                if (j < 8 || n0_of + c + 8 < g.N) top = fmaxf(top, fabsf(v[j]));
+                r[j] = __float_as_uint(v[j]);
+              }
+              tmem_st16(taddr + c - c0, r);
+            }
+          }
+          if (narrow) {
+            tmem_wait_st();
+            row_top = top;
+          }
+          if constexpr (BN == 256) {  // (a thread has a whole group)
+            if (narrow) {
+              const float s = block_scale(row_top, args.pow2 != 0), inv = __frcp_rn(s);
+              const int block = n0_of / 128 + group;
+              if (live && block < nb) args.c_scale[static_cast<size_t>(block) * g.M + m] = s;
+              uint8_t* c_row = static_cast<uint8_t*>(g.C) + static_cast<size_t>(m) * g.N;
+              const bool wide = g.N % 16 == 0;
+#pragma unroll 1
+              for (int c = group * kCols; c < (group + 1) * kCols; c += 16) {
+                const int n = n0_of + c;
+                if (n >= g.N) break;
+                uint32_t r[16], w[4];
+                tmem_ld16(taddr + c - group * kCols, r);
+                tmem_wait_ld_into(r);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  w[j] = pack_e4m3x4(__fmul_rn(__uint_as_float(r[4 * j]), inv), __fmul_rn(__uint_as_float(r[4 * j + 1]), inv), __fmul_rn(__uint_as_float(r[4 * j + 2]), inv),
+                                     __fmul_rn(__uint_as_float(r[4 * j + 3]), inv));
+                if (!live) continue;
+                if (wide) {
+                  *reinterpret_cast<uint4*>(c_row + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                  *reinterpret_cast<uint2*>(c_row + n) = make_uint2(w[0], w[1]);
+                  if (n + 8 < g.N) *reinterpret_cast<uint2*>(c_row + n + 8) = make_uint2(w[2], w[3]);
+                }
               }
             }
           }
         }
       }
+      release(last_buf);
+      if (!ok) break;
     }
   }
 
@@ -439,11 +561,14 @@ static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
       const int kbps = (kb_total + s - 1) / s;
       if ((kb_total + kbps - 1) / kbps != s || (s > 1 && p.split_k == 0 && kbps < 4)) continue;
       const long tiles = static_cast<long>(row_tiles) * ((p.N + bn - 1) / bn);
+      // Measured: ns per block of K (more where the operands of over a hundred CTAs share the way out of L2), what a tile adds, and the
+      // set-up of a launch.  Slices add their exchange, which grows with the CTAs that push at once.
       const long slots = s == 4 ? 33 : s == 8 ? 15 : sms / s;  // clusters that run at once
       const long rounds = (tiles + slots - 1) / slots;
-      const double body = kbps * (bn == 64 ? 165.0 : bn == 128 ? 215.0 : 300.0);
-      double cost = 3500.0 + bn * 4.0 + body + (rounds - 1) * (body + 2500.0 + bn * 4.0);
-      if (s > 1) cost += 300.0 + 12.0 * tiles * s;
+      const bool busy = tiles * s > 100;
+      const double per_kb = bn == 64 ? 195.0 : bn == 128 ? (busy ? 290.0 : 230.0) : (busy ? 600.0 : 530.0);
+      double cost = 3500.0 + rounds * (kbps * per_kb + 600.0 + 4.0 * bn + (bn == 256 && p.c_dtype == QB_E4M3 ? 2500.0 : 0.0));
+      if (s > 1) cost += 300.0 + 12.0 * tiles * s + (rounds - 1) * 4000.0;
       if (cost < best_cost) {
         best_cost = cost;
         best = BlockPlan{bn, s, kb_total, kbps};
@@ -500,7 +625,6 @@ static int32_t validate_blocks(const qb_gemm_blocks_params* p) {
   QB_REQUIRE(p->activation == 0 || p->activation == 1, QB_ERR_INVALID_ARG, "gemm_blocks: activation %d", p->activation);
   QB_REQUIRE(p->tile_n == 0 || p->tile_n == 64 || p->tile_n == 128 || p->tile_n == 256, QB_ERR_INVALID_ARG, "gemm_blocks: tile_n %d", p->tile_n);
   QB_REQUIRE(p->split_k >= 0 && p->split_k <= 8, QB_ERR_INVALID_ARG, "gemm_blocks: split_k %d", p->split_k);
-  QB_REQUIRE(p->M <= 65535 * kBM, QB_ERR_INVALID_ARG, "gemm_blocks: %d rows", p->M);
   return QB_OK;
 }
 
@@ -526,7 +650,9 @@ static int32_t blocks_run(const void* A, const void* B, const float* a_scale, co
     g.rows_per_gate = p->M / p->gate_groups;
   }
   const int row_tiles = (p->M + kBM - 1) / kBM;
-  const BlockPlan pl = plan_blocks(*p, row_tiles);
+  // Grouped: the slots are what any routing fits; with few tokens an expert's run is one tile, with many it ends halfway in one.
+  const int used_tiles = !grouped ? row_tiles : 2 * row_tiles <= 3 * n_experts ? (row_tiles < n_experts ? row_tiles : n_experts) : row_tiles - n_experts / 2;
+  const BlockPlan pl = plan_blocks(*p, used_tiles);
   g.M = p->M; g.N = p->N; g.K = p->K;
   g.a_rows = p->M < kBM ? (p->M + 7) / 8 * 8 : kBM;
   g.kb_total = pl.kb_total; g.kb_per_split = pl.kb_per_split; g.splits = pl.splits; g.cluster = pl.splits > 1;
@@ -550,7 +676,11 @@ static int32_t blocks_run(const void* A, const void* B, const float* a_scale, co
   }
   rc = make_tmap_2d_sw(&tmB, B, 1, static_cast<uint64_t>(p->N) * n_experts, p->K, pl.bn, 128, 128);
   if (rc != QB_OK) return rc;
-  const dim3 grid((p->N + pl.bn - 1) / pl.bn, row_tiles, pl.splits);
+  g.tiles_m = row_tiles;
+  const long long n_tiles = static_cast<long long>(row_tiles) * ((p->N + pl.bn - 1) / pl.bn);
+  QB_REQUIRE(n_tiles < (1ll << 30), QB_ERR_INVALID_ARG, "gemm_blocks: %lld tiles", n_tiles);
+  g.n_tiles = static_cast<int>(n_tiles);
+  const dim3 grid(pl.splits > 1 || n_tiles < num_sms() ? g.n_tiles : num_sms(), 1, pl.splits);
   if (grouped) return pl.bn == 256 ? launch_blocks<256, true>(tmA, tmA_small, tmB, a, grid, st) : pl.bn == 128 ? launch_blocks<128, true>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, true>(tmA, tmA_small, tmB, a, grid, st);
   return pl.bn == 256 ? launch_blocks<256, false>(tmA, tmA_small, tmB, a, grid, st) : pl.bn == 128 ? launch_blocks<128, false>(tmA, tmA_small, tmB, a, grid, st) : launch_blocks<64, false>(tmA, tmA_small, tmB, a, grid, st);
 }
