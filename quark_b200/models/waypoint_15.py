@@ -91,6 +91,17 @@ class Waypoint15Config:
     # output channel (amax / 448), the caches with one scale per KV head (`k_scale` / `v_scale` of each block's
     # parameters).  Only meaningful where quant says fp8; the mixture-of-experts weights stay unscaled.
     fp8_scales: bool = False
+    # Block-scaled e4m3 (an extension): linear and expert weights narrowed with one scale per 128 x 128 tile, their activations with one per
+    # row and 128 channels.  Where quant says fp8; takes the place of fp8_scales for the linears (the caches keep theirs).
+    fp8_blocks: bool = False
+    # Routing by scores (an extension, see nn.MoE): None keeps the reference's "correct" routing.
+    moe_scoring: str | None = None
+    moe_n_groups: int = 1
+    moe_topk_groups: int = 1
+    moe_group_top: int = 1
+    moe_renormalize: bool = True
+    moe_route_scale: float = 1.0
+    moe_score_bias: bool = False
     # Tensor parallelism by KV-head group: rank `tp_rank` of `tp_world` owns n_kv_heads / tp_world KV heads
     # with their Q heads (QKV and fc1 column-parallel, out-proj and fc2 row-parallel, partial outputs summed
     # over the ranks).  The reference is single-GPU; tp_world = 1 is its wiring.
@@ -106,8 +117,12 @@ class Waypoint15Config:
             if self.tp_world > 1:
                 raise NotImplementedError("Waypoint15Config: MoE with tp_world > 1 is not implemented")
             # the router is a GEMM with one output column per expert: a multiple of 8 columns
-            if not (1 <= self.moe_top_k <= self.moe_n_experts <= 32) or self.moe_n_experts % 8 or (self.d_model * self.mlp_ratio) % (8 * self.moe_top_k):
+            if not (1 <= self.moe_top_k <= self.moe_n_experts <= (512 if self.moe_scoring else 32)) or self.moe_n_experts % 8 or (self.d_model * self.mlp_ratio) % (8 * self.moe_top_k):
                 raise ValueError(f"Waypoint15Config: moe_top_k {self.moe_top_k} of {self.moe_n_experts} experts over an MLP of {self.d_model * self.mlp_ratio}")
+            if self.fp8_blocks and self.quant.moe == "fp8" and (self.d_model % 128 or self.mlp_dim // self.moe_top_k % 128):
+                raise ValueError(f"Waypoint15Config: experts of {self.d_model} x {self.mlp_dim // self.moe_top_k} have no whole 128 x 128 tiles")
+        if self.fp8_blocks and self.tp_world > 1:
+            raise NotImplementedError("Waypoint15Config: fp8_blocks with tp_world > 1 is not implemented")
         q = self.quilt_factor
         if q < 1 or q & (q - 1) or (self.height * self.width) % q:
             raise ValueError(f"Waypoint15Config: quilt_factor {q} must be a power of two that divides height * width")
@@ -186,8 +201,8 @@ class Waypoint15Config:
 
     _YAML_SCALARS = ("d_model", "n_layers", "n_heads", "n_kv_heads", "mlp_ratio", "channels", "height", "width", "local_window",
                      "global_window", "global_pinned_dilation", "global_attn_period", "global_attn_offset", "value_residual",
-                     "fourier_dim", "n_buttons", "ctrl_conditioning_period", "moe", "moe_n_experts", "moe_top_k", "moe_routing",
-                     "quilt_factor")  # fmt: skip
+                     "fourier_dim", "n_buttons", "ctrl_conditioning_period", "moe", "moe_n_experts", "moe_top_k", "moe_routing", "moe_scoring",
+                     "moe_n_groups", "moe_topk_groups", "moe_group_top", "moe_renormalize", "moe_route_scale", "moe_score_bias", "quilt_factor")  # fmt: skip
 
     @classmethod
     def from_dict(cls, raw: dict, **overrides) -> "Waypoint15Config":
@@ -267,6 +282,8 @@ def make_params(cfg: Waypoint15Config, seed: int = 0, *, weight_std: float = 0.0
             blk["moe.router.weight"] = _randn_bf16(rm, (E, d), 10 * weight_std)  # spread logits, so routing is not a coin toss
             blk["moe.expert_in"] = _randn_bf16(rm, (E * Hm, d), weight_std)
             blk["moe.expert_out"] = _randn_bf16(rm, (E * d, Hm), weight_std)
+            if cfg.moe_score_bias:
+                blk["moe.score_bias"] = (0.05 * rm.standard_normal(E)).astype(np.float32)
         ab = _cond.bf16_to_f32(_randn_bf16(r, (d,), weight_std))
         mb = _cond.bf16_to_f32(_randn_bf16(r, (d,), weight_std))
         projs = [_cond.bf16_to_f32(_randn_bf16(r, (d, d), weight_std)) for _ in range(6)]
@@ -352,7 +369,9 @@ class TransformerBlock(nn.Module):
             self.ctrl_residual = nn.Add()
         self.pre_mlp_norm = nn.AdaRMSNorm(chained=True)
         if cfg.moe:
-            self.mlp = nn.MoE(cfg.tpf, d, cfg.mlp_dim // cfg.moe_top_k, cfg.moe_n_experts, cfg.moe_top_k, routing=cfg.moe_routing)
+            self.mlp = nn.MoE(cfg.tpf, d, cfg.mlp_dim // cfg.moe_top_k, cfg.moe_n_experts, cfg.moe_top_k, routing=cfg.moe_routing, scoring=cfg.moe_scoring,
+                              n_groups=cfg.moe_n_groups, topk_groups=cfg.moe_topk_groups, group_top=cfg.moe_group_top, renormalize=cfg.moe_renormalize,
+                              route_scale=cfg.moe_route_scale, score_bias=cfg.moe_score_bias)  # fmt: skip
         else:
             self.mlp = nn.MLP(d, cfg.mlp_dim_local, d, out_dtype="bf16", fuse_silu=cfg.fuse_silu)
         self.mlp_gate = nn.AdaGateResidual()
@@ -371,7 +390,8 @@ class TransformerBlock(nn.Module):
         previous block left there.  ``prefetch`` is called just before the attention is launched.  ``ctrl_row`` is what
         ``Waypoint15.ctrl_rows`` made of the controller embedding for this block; without it the block works it out."""
         s0, b0, g0, s1, b1, g1 = self._cond_lut[sigma_idx]
-        fp8 = self.qkv_proj.weight.data.dtype == "e4m3"
+        # what a linear's input is handed over in: block-scaled linears narrow theirs themselves
+        fp8 = self.qkv_proj.weight.data.dtype == "e4m3" and self.qkv_proj.w_blocks is None
         tp = self._cfg.tp_world > 1
         tp_fused = tp and getattr(self._comm, "fused", False)
         # row-parallel partial outputs are summed over the ranks before gate and residual are applied (once)
@@ -387,7 +407,7 @@ class TransformerBlock(nn.Module):
         quilted = self._cfg.quilt_factor > 1
         kc = self.kv_cache
         quilt_fits = self._cfg.quilt_factor * (16 if kc.K_cache.dtype == "e4m3" else 8) <= 128
-        if self._cfg.fuse_qkv_post and self._cfg.fuse_qkv_gemm and quilt_fits:
+        if self._cfg.fuse_qkv_post and self._cfg.fuse_qkv_gemm and quilt_fits and self.qkv_proj.w_blocks is None:
             kc = self.kv_cache
             qkv = qf.gemm_qkv_post(
                 h0, self.qkv_proj.weight.data, qkv_first if use_first else None, self.v_residual.lamb.data if use_first else None,
@@ -493,6 +513,8 @@ class Waypoint15(nn.Module):
                 blk.mlp.router.weight.data = up(p["moe.router.weight"])
                 blk.mlp.expert_in.data = up(p["moe.expert_in"])
                 blk.mlp.expert_out.data = up(p["moe.expert_out"])
+                if self.cfg.moe_score_bias:
+                    blk.mlp.score_bias.data = QuarkTensor.from_numpy(np.asarray(p["moe.score_bias"], dtype=np.float32))
             else:
                 blk.mlp.fc1.weight.data = up(p["fc1.weight"])
                 blk.mlp.fc2.weight.data = up(p["fc2.weight"])
@@ -511,11 +533,12 @@ class Waypoint15(nn.Module):
         """Quantise linear weights when ``cfg.quant.linear == "fp8"`` (``waypoint_15.py:502-535``)."""
         kwargs.setdefault("fp8", self.cfg.quant.linear == "fp8")
         kwargs.setdefault("fp8_scaled", self.cfg.fp8_scales)
+        kwargs.setdefault("fp8_blocks", self.cfg.fp8_blocks)
         for blk in self.blocks:
             for lin in (blk.qkv_proj, blk.out_proj) + (() if self.cfg.moe else (blk.mlp.fc1, blk.mlp.fc2)):
                 lin.prepare(**kwargs)
             if self.cfg.moe:  # the experts follow quant.moe, independently of the other linears (waypoint_15.py:505-517)
-                blk.mlp.prepare(moe_fp8=self.cfg.quant.moe == "fp8")
+                blk.mlp.prepare(moe_fp8=self.cfg.quant.moe == "fp8", fp8_blocks=self.cfg.fp8_blocks)
         _stream.synchronize()
 
     def encode_ctrl(self, ctrl_input):

@@ -126,16 +126,20 @@ class Linear(Module):
         self._fp8_skip = fp8_skip
         self._fp8 = False
         self.w_scale = None  # f32 [out_features] after prepare(fp8=True, fp8_scaled=True)
+        self.w_blocks = None  # f32 [ceil(out_features / 128), ceil(in_features / 128)] after prepare(fp8=True, fp8_blocks=True)
         if bias:
             self.bias = Parameter(QuarkTensor.zeros(out_features, dtype="bf16"))
 
-    def prepare(self, *, shuffle: bool = False, fp8: bool = False, fp8_scaled: bool = False, **kwargs):
+    def prepare(self, *, shuffle: bool = False, fp8: bool = False, fp8_scaled: bool = False, fp8_blocks: bool = False, **kwargs):
         """``fp8_scaled`` (extension): narrow with one scale per output channel (``amax / 448``) instead of unscaled;
-        the scales stay with the layer and are applied in the GEMM's epilogue."""
+        the scales stay with the layer and are applied in the GEMM's epilogue.  ``fp8_blocks`` (extension): narrow with one scale
+        per 128 x 128 tile; the activations are then narrowed with one per row and 128 channels (``qf.gemm_blocks``)."""
         if shuffle:
             raise RuntimeError("weight shuffling is not supported (it is disabled upstream as well)")
         if fp8 and not self._fp8_skip and not self._fp8:
-            if fp8_scaled:
+            if fp8_blocks:
+                self.weight.data, self.w_blocks = qf.quantize_e4m3_blocks(self.weight.data, tile_rows=qf.BLOCK)
+            elif fp8_scaled:
                 self.weight.data, self.w_scale = qf.quantize_e4m3_rows(self.weight.data)
             else:
                 self.weight.data = qf.quantize_e4m3(self.weight.data)
@@ -143,7 +147,12 @@ class Linear(Module):
 
     def forward(self, x, *, activation=None, bias=None, gate=None, residual=None, gate_groups: int = 1, out_dtype=None, out=None, tp_arena=None):
         """``tp_arena``: a row-parallel linear of a tensor-parallel rank; the partial output is stored straight into the
-        staging areas of the ranks that sum it (``qf.gemm_tp``) and nothing is returned."""
+        staging areas of the ranks that sum it (``qf.gemm_tp``) and nothing is returned.
+
+        With block scales ``x`` may be a pair ``(e4m3, scales)`` as ``qf.quantize_e4m3_blocks`` returns it, and ``out_dtype="e4m3"`` returns
+        such a pair."""
+        if self.w_blocks is not None:
+            return self._forward_blocks(x, activation, bias, gate, residual, gate_groups, out_dtype, out, tp_arena)
         a_dt = x.dtype
         if tp_arena is not None:
             if activation is not None or bias is not None or gate is not None or self._has_bias or self.w_scale is not None:
@@ -173,6 +182,28 @@ class Linear(Module):
         )  # fmt: skip
 
 
+    def _forward_blocks(self, x, activation, bias, gate, residual, gate_groups, out_dtype, out, tp_arena):
+        if tp_arena is not None:
+            raise ValueError("Linear: a partial output sent to its reducers takes no block scales")
+        if self._has_bias and bias is not None:
+            raise ValueError("Linear: call-time bias= conflicts with a layer constructed with bias=True")
+        if not isinstance(x, tuple):
+            if x.dtype not in ("bf16", "f32"):
+                raise TypeError(f"Linear: a {x.dtype!r} activation without scales for a block-scaled weight (bf16, f32 or a pair)")
+            K = int(x.shape[-1])
+            M = x.numel // K
+            x = qf.quantize_e4m3_blocks(x, out=_cached(self, "xq", (M, K), "e4m3"), scale_out=_cached(self, "xs", (-(-K // qf.BLOCK), M), "f32"))
+        M, N = x[0].numel // int(x[0].shape[-1]), int(self.weight.data.shape[0])
+        od = out_dtype or self._out_dtype
+        if out is None:
+            out = _cached(self, "out", (M, N), od)
+        return qf.gemm_blocks(
+            x[0], self.weight.data, x[1], self.w_blocks, out_dtype=od, activation=activation, bias=self.bias.data if self._has_bias else bias, gate=gate,
+            residual=residual, gate_groups=gate_groups, out=out, scale_out=_cached(self, "out_s", (-(-N // qf.BLOCK), M), "f32") if od == "e4m3" else None,
+            b_constant=True,
+        )  # fmt: skip
+
+
 class MoE(Module):
     """Top-k mixture of expert MLPs, ``routing="correct"`` of the reference (``src/quark/nn/moe.py:103-363``): every
     token goes to its own ``top_k`` experts with a softmax over their logits as weights,
@@ -186,26 +217,57 @@ class MoE(Module):
     ``schedule="dense"`` keeps the earlier form (every expert over every token, routing weights zero outside a token's
     top k: E / top_k times the flops, no data-dependent tables; the same bits as long as its products take one K slice, else another
     order of the f32 sums).  The capacity-bounded ``"balanced"`` and
-    ``"shared_experts"`` routings are rejected, as upstream's own ``forward`` does (``src/quark/nn/moe.py:340-347``)."""
+    ``"shared_experts"`` routings are rejected, as upstream's own ``forward`` does (``src/quark/nn/moe.py:340-347``).
+
+    Extensions: ``scoring`` (``"softmax"`` or ``"sigmoid"``) routes by ``qf.moe_route_scored`` on f32 logits, up to 512 experts, with its ``n_groups``,
+    ``topk_groups``, ``group_top``, ``renormalize`` and ``route_scale`` (its ``factor``); ``score_bias`` gives the layer a parameter of that name, f32
+    ``[E]``, that takes part in the choice.  ``prepare(fp8_blocks=True)`` narrows the experts' weights with a scale per 128 x 128 tile and
+    the activations with one per row and 128 channels (``qf.gemm_grouped_blocks``); both widths are then multiples of 128."""
 
     def __init__(self, M: int, d_model: int, d_intermediate: int, n_experts: int, top_k: int, *, routing: str = "correct", out_dtype: str = "bf16",
-                 schedule: str = "sorted"):  # fmt: skip
+                 schedule: str = "sorted", scoring: str | None = None, n_groups: int = 1, topk_groups: int = 1, group_top: int = 1,
+                 renormalize: bool = True, route_scale: float = 1.0, score_bias: bool = False):  # fmt: skip
         if routing != "correct":
             raise NotImplementedError(f"MoE: routing {routing!r} is not implemented (only 'correct')")
         if schedule not in ("sorted", "dense"):
             raise ValueError(f"MoE: schedule {schedule!r} (sorted or dense)")
-        if not (1 <= top_k <= n_experts <= 32) or n_experts % 8:
-            raise ValueError(f"MoE: top_k {top_k} of {n_experts} experts (8, 16, 24 or 32: the router is a GEMM with one column per expert)")
+        if scoring is None:
+            if not (1 <= top_k <= n_experts <= 32) or n_experts % 8:
+                raise ValueError(f"MoE: top_k {top_k} of {n_experts} experts (8, 16, 24 or 32: the router is a GEMM with one column per expert)")
+            if n_groups != 1 or not renormalize or route_scale != 1.0 or score_bias:
+                raise ValueError("MoE: groups, a factor, a bias and weights as they are go with scoring=")
+        elif scoring not in ("softmax", "sigmoid") or schedule != "sorted":
+            raise ValueError(f"MoE: scoring {scoring!r} (softmax or sigmoid), schedule {schedule!r} (sorted)")
+        elif not (1 <= top_k <= min(n_experts, 32)) or n_experts > 512 or n_experts % 8:
+            raise ValueError(f"MoE: top_k {top_k} (at most 32) of {n_experts} experts (a multiple of 8, at most 512)")
+        elif not (1 <= topk_groups <= n_groups <= 32) or n_experts % n_groups or topk_groups * (n_experts // n_groups) < top_k:
+            raise ValueError(f"MoE: {topk_groups} of {n_groups} groups of experts for top_k {top_k} of {n_experts}")
+        elif group_top not in (1, 2) or (n_groups > 1 and n_experts // n_groups < group_top):
+            raise ValueError(f"MoE: group_top {group_top} of groups of {n_experts // n_groups}")
         self._M, self._D, self._H, self._E, self._K = M, d_model, d_intermediate, n_experts, top_k
         self._schedule = schedule
-        self.router = Linear(d_model, n_experts, out_dtype="bf16", fp8_skip=True)  # stays bf16: few columns, precision matters
+        self._scoring = scoring
+        self._route = dict(scoring=scoring or "softmax", n_groups=int(n_groups), topk_groups=int(topk_groups), group_top=int(group_top), renormalize=bool(renormalize),
+                           factor=float(route_scale))  # fmt: skip
+        self.router = Linear(d_model, n_experts, out_dtype="f32" if scoring else "bf16", fp8_skip=True)  # bf16 weights: few columns, precision matters
+        if score_bias:
+            self.score_bias = Parameter(QuarkTensor.zeros(n_experts, dtype="f32"))
         self.expert_in = Parameter(QuarkTensor.zeros(n_experts * d_intermediate, d_model, dtype="bf16"))
         self.expert_out = Parameter(QuarkTensor.zeros(n_experts * d_model, d_intermediate, dtype="bf16"))
         self._fp8 = False
+        self._blocks = None  # the experts' scales after prepare(fp8_blocks=True)
 
-    def prepare(self, *, fp8: bool = False, moe_fp8: bool | None = None, **kwargs):
+    def prepare(self, *, fp8: bool = False, moe_fp8: bool | None = None, fp8_blocks: bool = False, **kwargs):
         use = fp8 if moe_fp8 is None else moe_fp8
-        if use and not self._fp8:
+        if use and fp8_blocks and not self._fp8:
+            if self._schedule != "sorted" or self._D % qf.BLOCK or self._H % qf.BLOCK:
+                raise ValueError(f"MoE: block scales need the sorted schedule and widths that are multiples of 128, got {self._D} and {self._H}")
+            self._blocks = []
+            for p in (self.expert_in, self.expert_out):  # (every expert has whole tiles of its own)
+                p.data, scale = qf.quantize_e4m3_blocks(p.data, tile_rows=qf.BLOCK)
+                self._blocks.append(scale)
+            self._fp8 = True
+        elif use and not self._fp8:
             self.expert_in.data = qf.quantize_e4m3(self.expert_in.data)
             self.expert_out.data = qf.quantize_e4m3(self.expert_out.data)
             self._fp8 = True
@@ -214,6 +276,8 @@ class MoE(Module):
         M, D, H, E = x.numel // int(x.shape[-1]), self._D, self._H, self._E
         cd = "e4m3" if self._fp8 else None
         logits = self.router(x)
+        if self._scoring or self._blocks:
+            return self._forward_scored(x, logits, M)
         if self._schedule == "sorted":
             n = qf.moe_slots(M, E, self._K)
             slot_token, slot_weight, tile_expert, token_slot = qf.moe_route_slots(
@@ -246,6 +310,29 @@ class MoE(Module):
         return qf.moe_combine(partials, weights, out=_cached(self, "out", (M, D), "bf16"))
 
 
+    def _forward_scored(self, x, logits, M):
+        # (without scoring: a softmax over the top k logits is the renormalised softmax over all)
+        D, H, E, K = self._D, self._H, self._E, self._K
+        n = qf.moe_scored_slots(M, E, K)
+        shapes = (("experts", (M, K), "s32"), ("weights", (M, K), "f32"), ("slot_token", (n,), "s32"), ("slot_weight", (n,), "f32"), ("tile_expert", (n // 128,), "s32"),
+                  ("tile_rows", (n // 128,), "s32"), ("token_slot", (M, K), "s32"))  # fmt: skip
+        bias = self.score_bias.data if hasattr(self, "score_bias") else None
+        r = qf.moe_route_scored(logits, bias, top_k=K, out=[_cached(self, *t) for t in shapes], **self._route)
+        partials = _cached(self, "partials_s", (n, D), "f32")
+        if self._blocks:
+            xs = qf.quantize_e4m3_blocks(x, row_index=r.slot_token, out=_cached(self, "xs", (n, D), "e4m3"), scale_out=_cached(self, "xs_s", (D // qf.BLOCK, n), "f32"))
+            h = qf.gemm_grouped_blocks(xs[0], self.expert_in.data, xs[1], self._blocks[0], r.tile_expert, r.tile_rows, n_experts=E, activation="silu",
+                                       out=_cached(self, "h_s", (n, H), "e4m3"), scale_out=_cached(self, "h_ss", (H // qf.BLOCK, n), "f32"), b_constant=True)  # fmt: skip
+            qf.gemm_grouped_blocks(h[0], self.expert_out.data, h[1], self._blocks[1], r.tile_expert, r.tile_rows, n_experts=E, out=partials, b_constant=True)
+        else:
+            od, cd = ("e4m3", "e4m3") if self._fp8 else ("bf16", None)
+            xs = qf.moe_gather(x, r.slot_token, out=_cached(self, "xs", (n, D), od))
+            h = qf.gemm_grouped(xs, self.expert_in.data, r.tile_expert, n_experts=E, out_dtype=od, compute_dtype=cd, activation="silu", out=_cached(self, "h_s", (n, H), od),
+                                b_constant=True, through_bf16=self._fp8)  # fmt: skip
+            qf.gemm_grouped(h, self.expert_out.data, r.tile_expert, n_experts=E, out_dtype="f32", compute_dtype=cd, out=partials, b_constant=True)
+        return qf.moe_reduce(partials, r.slot_weight, r.token_slot, out=_cached(self, "out", (M, D), "bf16"))
+
+
 class SiLU(Module):
     def forward(self, x, *, emit_e4m3: bool = False):
         out = _cached(self, "out", x.shape, x.dtype)
@@ -270,8 +357,10 @@ class MLP(Module):
 
     def forward(self, x, *, gate=None, residual=None, gate_groups: int = 1, out=None, tp_arena=None):
         fp8 = self.fc2.weight.data.dtype == "e4m3"
-        if self._fuse_silu:
+        if self._fuse_silu:  # (block scales: an e4m3 result comes with its scales)
             h = self.fc1(x, activation="silu", out_dtype="e4m3" if fp8 else None)
+        elif self.fc2.w_blocks is not None:
+            h = self.silu(self.fc1(x))
         else:
             h = self.silu(self.fc1(x), emit_e4m3=fp8)
         if tp_arena is not None:
