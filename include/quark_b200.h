@@ -431,7 +431,7 @@ typedef struct {
   int32_t pow2;        /* e4m3 C: scales that are powers of two */
   int32_t b_constant;  /* as bit 1 of qb_gemm_params.reserved; covers b_scale too */
   int32_t tile_n;      /* 0 = choose; 64, 128 or 256 (an e4m3 C: 128 or 256) */
-  int32_t split_k;     /* 0 = choose; 1, 2, 4 or 8 K slices (more than one: tiles of 64 columns) */
+  int32_t split_k;     /* 0 = choose; 1, 2, 4 or 8 K slices (more than one: tiles of 64 columns, not grouped; one where K has too few blocks) */
 } qb_gemm_blocks_params;
 int32_t qb_gemm_blocks(const void* A, const void* B, const float* a_scale, const float* b_scale, void* C, float* c_scale, const void* bias, const void* gate,
                        const void* residual, const qb_gemm_blocks_params* p, void* stream);

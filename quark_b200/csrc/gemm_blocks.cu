@@ -550,6 +550,8 @@ struct BlockPlan {
 // Width of the tiles and number of K slices.
 static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
   const int kb_total = (p.K + 127) / 128, sms = num_sms();
+  auto slices = [&](int s) { return (kb_total + (kb_total + s - 1) / s - 1) / ((kb_total + s - 1) / s) == s; };  // every one has a block
+  const int asked = p.split_k > 1 && !slices(p.split_k) ? 1 : p.split_k;
   BlockPlan best{128, 1, kb_total, kb_total};
   double best_cost = 1e30;
   for (int bn = 64; bn <= 256; bn *= 2) {
@@ -557,9 +559,9 @@ static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
     if (p.c_dtype == QB_E4M3 && bn == 64) continue;  // a group of 128 results is one tile's
     if (bn > 64 && p.tile_n == 0 && p.N <= bn / 2 && !(p.c_dtype == QB_E4M3 && bn == 128)) continue;
     for (int s = 1; s <= (bn == 64 ? 8 : 1); s *= 2) {
-      if (p.split_k != 0 && p.split_k != s) continue;
+      if (asked != 0 && asked != s) continue;
       const int kbps = (kb_total + s - 1) / s;
-      if ((kb_total + kbps - 1) / kbps != s || (s > 1 && p.split_k == 0 && kbps < 4)) continue;
+      if (!slices(s) || (s > 1 && asked == 0 && kbps < 4)) continue;
       const long tiles = static_cast<long>(row_tiles) * ((p.N + bn - 1) / bn);
       // Measured: ns per block of K (more where the operands of over a hundred CTAs share the way out of L2), what a tile adds, and the
       // set-up of a launch.  Slices add their exchange, which grows with the CTAs that push at once.
@@ -624,7 +626,10 @@ static int32_t validate_blocks(const qb_gemm_blocks_params* p) {
   QB_REQUIRE(p->N % 8 == 0, QB_ERR_ALIGN, "gemm_blocks: N = %d must be a multiple of 8", p->N);
   QB_REQUIRE(p->activation == 0 || p->activation == 1, QB_ERR_INVALID_ARG, "gemm_blocks: activation %d", p->activation);
   QB_REQUIRE(p->tile_n == 0 || p->tile_n == 64 || p->tile_n == 128 || p->tile_n == 256, QB_ERR_INVALID_ARG, "gemm_blocks: tile_n %d", p->tile_n);
-  QB_REQUIRE(p->split_k >= 0 && p->split_k <= 8, QB_ERR_INVALID_ARG, "gemm_blocks: split_k %d", p->split_k);
+  QB_REQUIRE(p->split_k >= 0 && p->split_k <= 8 && (p->split_k & (p->split_k - 1)) == 0, QB_ERR_INVALID_ARG, "gemm_blocks: split_k %d", p->split_k);
+  const bool wide = p->c_dtype == QB_E4M3 || p->tile_n > 64;  // (a group of 128 results is one tile's)
+  QB_REQUIRE(p->split_k <= 1 || !wide, QB_ERR_UNSUPPORTED, "gemm_blocks: K slices go with tiles of 64 columns and a bf16 or f32 result");
+  QB_REQUIRE(p->tile_n != 64 || !wide, QB_ERR_UNSUPPORTED, "gemm_blocks: an e4m3 result goes with tiles of 128 or 256 columns");
   return QB_OK;
 }
 
@@ -699,6 +704,7 @@ extern "C" int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const fl
   QB_REQUIRE(p != nullptr && tile_expert != nullptr && tile_rows != nullptr, QB_ERR_INVALID_ARG, "gemm_grouped_blocks: params or tile tables are NULL");
   QB_REQUIRE(p->M > 0 && p->M % kBM == 0, QB_ERR_UNSUPPORTED, "gemm_grouped_blocks: M = %d must be a multiple of 128", p->M);
   QB_REQUIRE(n_experts >= 1 && static_cast<long long>(n_experts) * p->N < (1ll << 31), QB_ERR_INVALID_ARG, "gemm_grouped_blocks: %d experts", n_experts);
+  QB_REQUIRE(p->split_k <= 1, QB_ERR_UNSUPPORTED, "gemm_grouped_blocks: split_k %d", p->split_k);
   qb_gemm_blocks_params q = *p;
   q.split_k = 1;  // a padding tile leaves before any K slice could wait for it
   return blocks_run(A, B, a_scale, b_scale, C, c_scale, nullptr, nullptr, nullptr, tile_expert, tile_rows, n_experts, &q, static_cast<cudaStream_t>(stream));

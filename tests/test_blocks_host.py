@@ -43,13 +43,16 @@ def test_entry_points_refuse_on_the_host():
     assert gemm(tile_n=96) == -1 and gemm(split_k=9) == -1 and gemm(A=None) == -1 and gemm(sa=None) == -1 and gemm(sb=None) == -1
     assert gemm(gate=ONE) == -1 and gemm(sc=ONE) == -1 and gemm(c_dtype=1) == -1 and "scales" in last()
     assert gemm(B=C.c_void_p(8)) == -3 and gemm(sb=C.c_void_p(2)) == -3
+    # a tile and slices that do not go together are no silent choice of others
+    assert gemm(split_k=3) == -1 and gemm(split_k=2, tile_n=128) == -2 and gemm(split_k=2, c_dtype=1, sc=ONE) == -2 and "64 columns" in last()
+    assert gemm(tile_n=64, c_dtype=1, sc=ONE) == -2
 
     def grouped(te=ONE, tr=ONE, experts=2, **kw):
         p = _lib.GemmBlocksParams(**{**dict(M=128, N=16, K=32, c_dtype=0, activation=0, gate_groups=1), **kw})
         return lib.qb_gemm_grouped_blocks(ONE, ONE, ONE, ONE, ONE, None, te, tr, experts, C.byref(p), None)
 
     assert grouped(te=None) == -1 and grouped(tr=None) == -1 and grouped(experts=0) == -1 and grouped(M=100) == -2 and grouped(M=0) == -2
-    assert grouped(experts=1 << 30) == -1
+    assert grouped(experts=1 << 30) == -1 and grouped(split_k=2) == -2
 
     def route(logits=ONE, bias=None, experts=ONE, weights=ONE, tabs=(ONE,) * 5, ws=None, ws_bytes=0, **kw):
         p = _lib.RouteParams(**{**dict(M=4, E=16, top_k=2, logits_dtype=2, scoring=0, n_groups=1, topk_groups=1, group_top=1, renormalize=1, factor=1.0), **kw})
