@@ -11,7 +11,11 @@
 //
 // A warp takes a token; its lanes hold P consecutive experts each.  The tables need, for every choice, how many earlier tokens chose
 // the same expert: a block's tokens are a 64-bit mask per expert (rank = set bits below the token), and blocks are joined by the
-// counts (a byte each) that they leave in the workspace.  Up to 64 tokens one block does all in one launch.
+// counts (a byte each) that they leave in the workspace.  A few tokens are one block's, which does all in one launch.
+//
+// What bounds it: a token of 256 experts in 8 groups is about 1100 instructions, so 8192 tokens take 16.1 us of issue slots (9.2 us 2048); among 512 or more
+// there is likely one whose choice needs the 64 bits, 3.7 us that nothing hides.  The tables add 3.7 - 8 us, a chain of trips to L2.  Every block adds
+// up the counts of all, which past 10,000 tokens grows with their square (65536 tokens: 70 of 170 us).
 #include <atomic>
 
 #include "common.cuh"
@@ -19,7 +23,7 @@
 namespace qb {
 
 constexpr int kRouteMaxExperts = 512, kRouteMaxGroups = 32, kRouteMaxTopK = 32;
-constexpr int kRouteTokens = 64;    // tokens of a block
+constexpr int kRouteTokens = 64, kRouteFewTokens = 4;  // most and fewest tokens of a block
 constexpr int kRouteThreads = 1024;
 constexpr int kRouteTile = 128;     // row tile of the grouped product
 constexpr size_t kRouteWsOffset = 64u << 10;  // the area in front belongs to the GEMM's counters
@@ -32,9 +36,12 @@ struct RouteArgs {
   int *experts, *slot_token, *tile_expert, *tile_rows, *token_slot;
   float *weights, *slot_weight;
   int n_tiles;
+  int tokens;       // of a block
   uint8_t* counts;  // [block][E rounded up to 4]
   int vec, vec_bias;  // rows of logits, and the bias, are whole 16-byte vectors
+  int size;     // experts of a group
   int regular;  // no groups, or groups of whole lanes, a power of two of them
+  int lanes;    // of a group then
 };
 
 // Unsigned keys in the order of the values; 0 is kept for what cannot be chosen, NaN comes next.
@@ -63,7 +70,7 @@ template <int P, typename V>
 __device__ __noinline__ int select_exact(const RouteArgs& a, const V (&c)[P], V* scratch) {
   const int lane = threadIdx.x & 31, e0 = lane * P;
   unsigned kept = 0xffffffffu;  // groups
-  const int size = a.E / a.groups;
+  const int size = a.size;
   if (a.groups > 1) {
     V best = lowest<V>(), second = lowest<V>();
 #pragma unroll
@@ -155,7 +162,7 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
         }
   bool fine = true;
   if (a.groups > 1) {
-    const int lanes = a.E / a.groups / P;  // of a group: a power of two
+    const int lanes = a.lanes;
     float best = value(key[0]), second = P > 1 ? value(key[P > 1 ? 1 : 0]) : __uint_as_float(0xff800000u);
     for (int o = 1; o < lanes; o <<= 1) {
       const float b = __shfl_xor_sync(0xffffffffu, best, o), s = __shfl_xor_sync(0xffffffffu, second, o);
@@ -175,7 +182,7 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
         break;
       }
       last = x;
-      if (lane / lanes == who / lanes) {
+      if ((lane ^ who) < lanes) {  // the same group
         mine_kept = true;
         open = 0u;
       }
@@ -185,15 +192,16 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
       for (int i = 0; i < P; ++i) key[i] = 0u;
     }
   }
-  const int left = a.groups == 1 ? a.E : a.kept * (a.E / a.groups);
+  const int left = a.groups == 1 ? a.E : a.kept * a.size;
   // top_k choices and the next one or two, as far as there are lanes and experts for them; lane j keeps the j-th and its key
   const int rounds = min(min(a.top_k + (kMargin ? 2 : 1), left), 32);
   mine = 0;
   uint32_t got = 0u;
   for (int j = 0; j < rounds; ++j) {
-    const uint32_t head = key[0] & ~kLow, most = __reduce_max_sync(0xffffffffu, head);
+    // (with kMargin, whichever of two equal values comes first: they are too close to count)
+    const uint32_t head = kMargin ? key[0] : key[0] & ~kLow, most = __reduce_max_sync(0xffffffffu, head);
     const int who = __ffs(__ballot_sync(0xffffffffu, head == most)) - 1;
-    const int e = __shfl_sync(0xffffffffu, e0 + static_cast<int>(kLow - (key[0] & kLow)), who);
+    const int e = kMargin ? who * P + static_cast<int>(kLow - (most & kLow)) : __shfl_sync(0xffffffffu, e0 + static_cast<int>(kLow - (key[0] & kLow)), who);
     if (lane == j) {
       mine = e;
       got = most;
@@ -305,7 +313,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
     if (found != kFound) {
       double sum = 0.0;
       if (!a.sigmoid) {
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < P; ++i) sum += exp(static_cast<double>(l[i]) - static_cast<double>(top));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -332,7 +340,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
         my_expert = sorted;
       } else {
         double d[P];
-#pragma unroll 1
+#pragma unroll  // (else the logits lie in local memory from the start: 8192 tokens 25.3 us instead of 24.2)
         for (int i = 0; i < P; ++i) d[i] = e0 + i < a.E ? score(l[i], e0 + i) : 0.0;
         my_expert = select_exact<P, double>(a, d, scratch);
       }
@@ -414,7 +422,7 @@ __device__ __forceinline__ void write_tables(const RouteArgs& a, RouteShared& sh
 }
 
 __device__ __forceinline__ void clear_shared(RouteShared& sh) {
-  for (int e = threadIdx.x; e < kRouteMaxExperts; e += kRouteThreads) sh.mask[e][0] = sh.mask[e][1] = sh.total[e] = sh.before[e] = 0;
+  for (int e = threadIdx.x; e < kRouteMaxExperts; e += blockDim.x) sh.mask[e][0] = sh.mask[e][1] = sh.total[e] = sh.before[e] = 0;
   __syncthreads();
 }
 
@@ -429,9 +437,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   grid_dep_launch();
   a.logits = after_wait(a.logits);
   a.bias = after_wait(a.bias);
-  const int t0 = blockIdx.x * kRouteTokens, tokens = min(a.M - t0, kRouteTokens);
+  const int t0 = blockIdx.x * a.tokens, tokens = min(a.M - t0, a.tokens);
   double* scratch = route_scratch + static_cast<size_t>(warp) * a.E;
-  for (int tl = warp; tl < tokens; tl += kRouteThreads / 32) {
+  for (int tl = warp; tl < tokens; tl += blockDim.x / 32) {
     int e;
     float w;
     choose<P, kScores>(a, t0 + tl, scratch, e, w);
@@ -444,10 +452,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   }
   if (a.n_tiles == 0) return;
   __syncthreads();
-  if (tid < a.E) {
-    const int n = __popc(sh.mask[tid][0]) + __popc(sh.mask[tid][1]);
-    if (gridDim.x > 1) a.counts[static_cast<size_t>(blockIdx.x) * ((a.E + 3) & ~3) + tid] = static_cast<uint8_t>(n);
-    sh.total[tid] = n;
+  for (int e = tid; e < a.E; e += blockDim.x) {
+    const int n = __popc(sh.mask[e][0]) + __popc(sh.mask[e][1]);
+    if (gridDim.x > 1) a.counts[static_cast<size_t>(blockIdx.x) * ((a.E + 3) & ~3) + e] = static_cast<uint8_t>(n);
+    sh.total[e] = n;
   }
   if (gridDim.x == 1) write_tables(a, sh, t0, tokens);
 }
@@ -461,7 +469,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_tables_kernel(const Route
   grid_dep_launch();
   a.experts = after_wait(a.experts);
   a.weights = after_wait(a.weights);
-  const int t0 = blockIdx.x * kRouteTokens, tokens = min(a.M - t0, kRouteTokens);
+  const int t0 = blockIdx.x * a.tokens, tokens = min(a.M - t0, a.tokens);
   for (int i = tid; i < tokens * a.top_k; i += kRouteThreads) {
     const int tl = i / a.top_k;
     atomicOr(&sh.mask[a.experts[static_cast<size_t>(t0) * a.top_k + i]][tl >> 5], 1u << (tl & 31));
@@ -497,8 +505,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_tables_kernel(const Route
 
 template <int P, bool kScores>
 static int32_t launch_choose(RouteArgs a, int blocks, cudaStream_t st) {
-  const int size = a.E / a.groups, lanes = size / P;
-  a.regular = a.groups == 1 || (size % P == 0 && (lanes & (lanes - 1)) == 0);
+  a.size = a.E / a.groups;
+  a.lanes = a.size / P;
+  a.regular = a.groups == 1 || (a.size % P == 0 && (a.lanes & (a.lanes - 1)) == 0);
   static std::atomic<unsigned long long> configured{0};  // one bit per device
   int dev = 0;
   QB_CUDA_OK(cudaGetDevice(&dev));
@@ -506,7 +515,8 @@ static int32_t launch_choose(RouteArgs a, int blocks, cudaStream_t st) {
     QB_CUDA_OK(cudaFuncSetAttribute(route_choose_kernel<P, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteThreads / 32 * P * 32 * 8));
     if (dev < 64) configured.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  return launch_dep("moe_route_scored", route_choose_kernel<P, kScores>, dim3(blocks), dim3(kRouteThreads), a.groups > 1 ? static_cast<size_t>(kRouteThreads / 32) * a.E * sizeof(double) : 0, st, a);
+  const int threads = blocks == 1 ? kRouteThreads : min(32 * a.tokens, kRouteThreads);  // (one block writes the tables as well)
+  return launch_dep("moe_route_scored", route_choose_kernel<P, kScores>, dim3(blocks), dim3(threads), a.groups > 1 ? static_cast<size_t>(threads / 32) * a.E * sizeof(double) : 0, st, a);
 }
 
 template <bool kScores>
@@ -518,6 +528,17 @@ static int32_t launch_choose(const RouteArgs& a, int blocks, cudaStream_t st) {
   if (per_lane <= 8) return launch_choose<8, kScores>(a, blocks, st);
   return launch_choose<16, kScores>(a, blocks, st);
 }
+
+// Tokens of a block, a warp to each up to 32.  Few, so that few warps share an SM's issue slots (512 tokens of 256 experts: 12.5 us with 16 to a block,
+// 12.1 with 8; 64 in one block, tables included: 19, in blocks of 4: 7.6), and as few blocks as that leaves, since every block of the tables
+// adds up the counts of all and waits for the others' lines (512 tokens: 14.2 us with 4 to a block).
+static int block_tokens(int M) {
+  int n = kRouteFewTokens;
+  while (n < 16 && (M + n - 1) / n > 64) n *= 2;
+  while (n < kRouteTokens && (M + n - 1) / n > 128) n *= 2;
+  return n;
+}
+static int route_blocks(int M) { return (M + block_tokens(M) - 1) / block_tokens(M); }
 
 static int32_t validate_route(const qb_route_params* p) {
   QB_REQUIRE(p != nullptr, QB_ERR_INVALID_ARG, "moe_route_scored: params are NULL");
@@ -548,8 +569,8 @@ extern "C" size_t qb_moe_scored_slots(int32_t M, int32_t E, int32_t top_k) {
 }
 
 extern "C" size_t qb_moe_route_scored_workspace_bytes(const qb_route_params* p) {
-  if (validate_route(p) != QB_OK || p->M <= kRouteTokens) return 0;
-  return kRouteWsOffset + static_cast<size_t>((p->M + kRouteTokens - 1) / kRouteTokens) * ((p->E + 3) & ~3);
+  if (validate_route(p) != QB_OK || route_blocks(p->M) == 1) return 0;
+  return kRouteWsOffset + static_cast<size_t>(route_blocks(p->M)) * ((p->E + 3) & ~3);
 }
 
 extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, int32_t* experts, float* weights, int32_t* slot_token, float* slot_weight, int32_t* tile_expert,
@@ -564,7 +585,7 @@ extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, in
                         reinterpret_cast<uintptr_t>(slot_weight) | reinterpret_cast<uintptr_t>(tile_expert) | reinterpret_cast<uintptr_t>(tile_rows) |
                         reinterpret_cast<uintptr_t>(token_slot);
   QB_REQUIRE(aligned16(logits) && (all & 3u) == 0, QB_ERR_ALIGN, "moe_route_scored: logits must be 16-byte aligned");
-  const int blocks = (p->M + kRouteTokens - 1) / kRouteTokens;
+  const int blocks = route_blocks(p->M);
   if (tables && blocks > 1) {
     const size_t need = qb_moe_route_scored_workspace_bytes(p);
     QB_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned16(workspace), QB_ERR_WORKSPACE, "moe_route_scored: workspace of %zu bytes needed, %zu given", need,
@@ -578,6 +599,7 @@ extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, in
   a.vec_bias = aligned16(bias) && a.E % 4 == 0;
   a.experts = experts; a.weights = weights; a.slot_token = slot_token; a.slot_weight = slot_weight; a.tile_expert = tile_expert; a.tile_rows = tile_rows;
   a.token_slot = token_slot;
+  a.tokens = block_tokens(p->M);
   a.n_tiles = tables ? static_cast<int>(qb_moe_scored_slots(p->M, p->E, p->top_k) / kRouteTile) : 0;
   a.counts = tables && blocks > 1 ? static_cast<uint8_t*>(workspace) + kRouteWsOffset : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -76,10 +76,11 @@ def test_sizes_of_the_slot_tables():
         n = M * k
         worst = max(sum(-(-c // 128) for c in ([1] * (u - 1) + [n - (u - 1)])) for u in range(1, min(E, n) + 1))
         assert lib.qb_moe_scored_slots(M, E, k) // 128 >= worst
-    p = _lib.RouteParams(M=64, E=256, top_k=8, logits_dtype=2, scoring=1, n_groups=8, topk_groups=4, group_top=2, renormalize=1, factor=1.0)
+    p = _lib.RouteParams(M=4, E=256, top_k=8, logits_dtype=2, scoring=1, n_groups=8, topk_groups=4, group_top=2, renormalize=1, factor=1.0)
     assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == 0
-    p.M = 129  # behind the area that belongs to the GEMM's tile counters
-    assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == (64 << 10) + 3 * 256
+    for M, counts in ((5, 2), (129, 33), (512, 64), (2048, 128), (8192, 128), (8193, 129)):  # behind the area that belongs to the GEMM's tile counters
+        p.M = M
+        assert lib.qb_moe_route_scored_workspace_bytes(C.byref(p)) == (64 << 10) + counts * 256
 
 
 @pytest.mark.parametrize("kind,call", [

@@ -388,6 +388,7 @@ def check_routing(got, e, w, E):
 @pytest.mark.parametrize("M,E,k,groups,kept,top", [
     (1, 8, 2, 1, 1, 1), (1, 256, 8, 8, 4, 2), (3, 1, 1, 1, 1, 1), (64, 64, 6, 8, 3, 1), (65, 160, 6, 8, 3, 2), (200, 96, 4, 4, 2, 2), (130, 40, 5, 8, 2, 1),
     (1000, 512, 32, 16, 8, 2), (2049, 256, 8, 8, 4, 2), (700, 16, 16, 1, 1, 1), (90, 300, 7, 30, 5, 2), (77, 512, 8, 32, 4, 1), (129, 264, 8, 4, 1, 2),
+    (4, 64, 6, 8, 4, 2), (5, 64, 6, 8, 4, 2), (513, 128, 3, 4, 2, 1), (8200, 64, 8, 8, 4, 2),  # tokens of a block: 4, 4, 16, 64
 ])  # fmt: skip
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("biased", [False, True])
