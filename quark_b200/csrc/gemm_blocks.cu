@@ -12,9 +12,12 @@
 //     the tensor core takes it (269 -> 150 - 190 without the sums);
 //   - the warps that sum took 865 with the scales loaded four blocks ahead (a load waits behind the operands, over 1000 clocks), 580 - 690
 //     with 16 warps of half the columns (what every warp does once a block filled the schedulers), and take 330 (64 columns) and 420 (128).
-// 24.5 -> 16.4 us and 28.3 -> 18.6 us at that size.
+// 24.5 -> 16.4 us (64) and 28.3 -> 18.6 us (128) at that size.  With all SMs at work the operands' way out of L2 is a bound beside it: a block of 128 columns, 32 KB a
+// CTA, takes 540 clocks then (13.4 TB/s).  256 columns, 840 clocks, need a quarter less of it and few CTAs' rounds: 4096^3 75 us in 128, 78 in 256 (1.8 PFLOP/s),
+// 8192^3 632 us in 256 (1.7 PFLOP/s, at the clock that the power limit leaves).
 //
-// A CTA stays for all tiles of its share: while its warps are in the epilogue of one, the copies and the MMAs of the next go on.
+// A CTA stays for all tiles of its share: while its warps are in the epilogue of one, the copies and the MMAs of the next go on (8192^3 814 -> 632 us,
+// 512 x 8192 x 2048 narrowed with SiLU 21.9 -> 17.4 with that, 256 columns and results narrowed from registers).
 // Warp 0 TMA, warp 1 MMA, warps 2-9 (4-11 with 256 columns) sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
 #include <atomic>
 
