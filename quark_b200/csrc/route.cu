@@ -127,14 +127,18 @@ __device__ __noinline__ int select_exact(const RouteArgs& a, const V (&c)[P], V*
 }
 
 // The same on values in 32 bits: a lane's experts become keys whose low bits hold their place in the lane, sorted once, and a round takes
-// the largest head.  kMargin: the values are off by less than 2^-20 of max(1, their size) each, low bits included (an exponential
-// of 2 ulp, a sum of at most 20 roundings, a quotient, the bias); without, they are exact but for the low bits.  What the whole warp learns:
+// the largest head.  kMargin: the values are off by less than kOff of max(1, their size) each, and a key lies below its value by up to kLow
+// units of its last place, kCut of its size.  (In units of 2^-24, a score being at most 1: an exponential 4; for softmax the P + 5
+// roundings of the sum, 13 with 8 experts to a lane, 21 with 16, and a quotient and a product 2; for the sigmoid a sum and a quotient 5; the
+// bias 1: 20 and 28, of the 24 and 32 that kOff is.)  Without, the values are exact but for the low bits.  What the whole warp learns:
 // kFound, kOrder (with kMargin: the choice is among the first top_k + 1, which lanes 0 .. top_k hold, but some of them lie within
-// 2^-18 of one another), or kOpen (too close for that, or equal with low bits lost: select_exact has to choose).
+// 2 kOff + kCut of one another), or kOpen (too close for that, or equal with low bits lost: select_exact has to choose).
 enum Selected { kFound, kOrder, kOpen };
 template <int P, bool kMargin>
 __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float (&c)[P], bool lossless, int& mine) {
   constexpr uint32_t kLow = P > 8 ? 15u : 7u;
+  constexpr float kOff = P > 8 ? 0x1p-19f : 0x1.8p-20f, kCut = static_cast<float>(kLow) * 0x1p-23f, kApart = P > 8 ? 0x1.8p-18f : 0x1p-18f;
+  static_assert(2.f * kOff + kCut < kApart, "see above");
   const int lane = threadIdx.x & 31, e0 = lane * P;
   uint32_t key[P];
 #pragma unroll
@@ -147,7 +151,7 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
     k &= ~kLow;
     return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
   };
-  auto apart = [](float hi, float lo) { return hi - lo > 0x1p-18f * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo))); };
+  auto apart = [](float hi, float lo) { return hi - lo > kApart * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo))); };
 #pragma unroll
   for (int size = 2; size <= P; size *= 2)  // descending, by a bitonic network
 #pragma unroll
@@ -172,20 +176,24 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
     const float score = a.top == 2 ? best + second : best;  // of this lane's group
     uint32_t open = lane * P < a.E ? order_key(score) : 0u;
     bool mine_kept = false;
-    float last = 0.f;
-    for (int j = 0; j <= a.kept; ++j) {  // (kept < groups)
-      const uint32_t most = __reduce_max_sync(0xffffffffu, open);
-      const int who = __ffs(__ballot_sync(0xffffffffu, open == most)) - 1;
-      const float x = __uint_as_float((most & 0x80000000u) ? most ^ 0x80000000u : ~most);
-      if (j == a.kept) {
-        fine = kMargin ? apart(last, x) : lossless || last != x;
-        break;
-      }
-      last = x;
+    uint32_t last = 0u;
+    for (int j = 0; j < a.kept; ++j) {  // (kept < groups)
+      last = __reduce_max_sync(0xffffffffu, open);
+      const int who = __ffs(__ballot_sync(0xffffffffu, open == last)) - 1;
       if ((lane ^ who) < lanes) {  // the same group
         mine_kept = true;
         open = 0u;
       }
+    }
+    if (kMargin) {
+      // A sum is off by what its terms are, which may be far larger than it: the lowest that any kept group's may be, against the highest
+      // of any other's.  (Minus infinity is exact, and as a bound NaN, the lowest key.)
+      const float size = a.top == 2 ? 2.f * fmaxf(fabsf(best), fabsf(second)) : fabsf(best), off = 2.f * kOff * fmaxf(1.f, size);
+      const uint32_t lo = mine_kept ? order_key(score - off) : 0xffffffffu;
+      const uint32_t hi = mine_kept || lane * P >= a.E ? 0u : order_key(score + (off + kCut * size));
+      fine = __reduce_min_sync(0xffffffffu, lo) > __reduce_max_sync(0xffffffffu, hi);
+    } else {
+      fine = lossless || last != __reduce_max_sync(0xffffffffu, open);
     }
     if (!mine_kept) {
 #pragma unroll

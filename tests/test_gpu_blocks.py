@@ -480,6 +480,20 @@ def test_routing_of_close_scores(qb, E, k, groups, kept, top, scoring, dense):
     check_routing(got, e, w, E)
 
 
+@pytest.mark.parametrize("E,groups,kept,k", [(16, 4, 2, 3), (64, 8, 3, 6), (256, 8, 4, 8), (512, 16, 5, 8), (40, 5, 2, 4)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_routing_of_groups_whose_best_two_cancel(qb, E, groups, kept, k, scoring):
+    """A group's best two values of large size and opposite sign: their sum is small, and what 32 bits lose of it goes by the size of the two."""
+    r = util.rng([19, E])
+    x = (1.5 * r.standard_normal((400, E))).astype(np.float32)
+    bias = np.full((groups, E // groups), -1e6, np.float32)
+    size = np.exp2(r.integers(4, 12, groups)).astype(np.float32)
+    bias[:, 1], bias[:, -1] = size, -size  # (exact in 64 bits beside a score)
+    bias = bias.reshape(-1)
+    got = qb.qf.moe_route_scored(T(qb, x), T(qb, bias), top_k=k, scoring=scoring, n_groups=groups, topk_groups=kept, group_top=2)
+    check_routing(got, *route(x, bias, k, scoring, groups, kept, 2), E)
+
+
 def test_routing_of_nan(qb):
     """NaN is chosen last, stays in its row, and never leads an index out of range."""
     r = util.rng(12)
