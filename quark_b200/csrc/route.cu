@@ -354,16 +354,31 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
       }
     }
   }
-  float s = 0.f;
+  float s = 0.f, x = 0.f;
   if (lane < a.top_k) {
-    const float x = logit_at(a, row, my_expert);
-    s = a.sigmoid ? 1.f / (1.f + expf(-x)) : expf(x - top);
+    x = logit_at(a, row, my_expert);
+    if (a.sigmoid) {
+      s = 1.f / (1.f + expf(-x));
+    } else {  // with what the difference was rounded by: far below the row's largest that is more than the rest
+      const float d = x - top, back = d - x, lost = (x - (d - back)) - (top + back);
+      s = expf(d);
+      if (s > 0.f) s = fmaf(s, lost, s);
+    }
   }
   float by = total;
   if (a.renorm) {
     by = s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) by += __shfl_xor_sync(0xffffffffu, by, o);
+    if (by < 1e-25f) {  // the bias chose experts whose scores leave 32 bits; their ratios do not
+      const double t = static_cast<double>(top);
+      const double wide = lane < a.top_k ? (a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - t)) : 0.0;
+      double all = wide;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      my_weight = all == 0.0 ? 0.f : static_cast<float>(wide / all) * a.factor;
+      return;
+    }
   }
   my_weight = by == 0.f ? 0.f : s / by * a.factor;
 }

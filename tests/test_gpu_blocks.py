@@ -494,6 +494,22 @@ def test_routing_of_groups_whose_best_two_cancel(qb, E, groups, kept, k, scoring
     check_routing(got, *route(x, bias, k, scoring, groups, kept, 2), E)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("low", [-40.0, -95.0, -150.0, -400.0])
+def test_weights_of_choices_with_tiny_scores(qb, scoring, low):
+    """The bias picks experts whose scores are far below the row's: what the weights are made of underflows in 32 bits, their ratios do not."""
+    r = util.rng([20, int(-low)])
+    x = r.standard_normal((70, 64)).astype(np.float32)
+    x[:, ::7] += np.float32(low)
+    bias = np.zeros(64, np.float32)
+    bias[::7] = 2.0 + np.arange(10)  # (apart, whatever the scores)
+    for k, renorm in ((1, True), (4, True), (10, True), (4, False)):
+        got = qb.qf.moe_route_scored(T(qb, x), T(qb, bias), top_k=k, scoring=scoring, renormalize=renorm)
+        e, w = route(x, bias, k, scoring, renorm=renorm)
+        assert np.all(e % 7 == 0)
+        check_routing(got, e, w, 64)
+
+
 def test_routing_of_nan(qb):
     """NaN is chosen last, stays in its row, and never leads an index out of range."""
     r = util.rng(12)
