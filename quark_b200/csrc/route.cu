@@ -13,9 +13,10 @@
 // the same expert: a block's tokens are a 64-bit mask per expert (rank = set bits below the token), and blocks are joined by the
 // counts (a byte each) that they leave in the workspace.  A few tokens are one block's, which does all in one launch.
 //
-// What bounds it: a token of 256 experts in 8 groups is about 1100 instructions, so 8192 tokens take 16.1 us of issue slots (9.2 us 2048); among 512 or more
-// there is likely one whose choice needs the 64 bits, 3.7 us that nothing hides.  The tables add 3.7 - 8 us, a chain of trips to L2.  Every block adds
-// up the counts of all, which past 10,000 tokens grows with their square (65536 tokens: 70 of 170 us).
+// What bounds it: a token of 256 experts in 8 groups is about 1100 instructions, so 8192 tokens take 13 us of issue slots (6.5 us 2048); among 512 or more
+// there is likely one with a comparison that needs the 64 bits, 1.5 us that nothing hides (3.7 with all of its scores in 64 bits instead of two to a lane:
+// 512 tokens 12.3 us with their tables instead of 9.6, 8192 24.9 instead of 20.9).  The tables add 3.7 - 8 us, a chain of trips to L2.  Every block adds up
+// the counts of all, which past 10,000 tokens grows with their square (65536 tokens: 70 of 170 us).
 #include <atomic>
 
 #include "common.cuh"
@@ -63,6 +64,33 @@ template <typename V>
 __device__ __forceinline__ V lowest() {
   return sizeof(V) == 8 ? static_cast<V>(__longlong_as_double(0xfff0000000000000ll)) : static_cast<V>(__uint_as_float(0xff800000u));
 }
+
+__device__ __forceinline__ float logit_at(const RouteArgs& a, const uint8_t* row, int e) {
+  return a.f32 ? reinterpret_cast<const float*>(row)[e] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[e]);
+}
+
+// What the formula compares, in 64 bits.
+struct Exact {
+  const RouteArgs& a;
+  const uint8_t* row;
+  float top;  // softmax: the largest logit
+  // softmax: 1 / the sum over the row, 0 for a row without one (the whole warp)
+  __device__ __forceinline__ double scale() const {
+    double sum = 0.0;
+    if (!a.sigmoid) {
+#pragma unroll 2
+      for (int e = threadIdx.x & 31; e < a.E; e += 32) sum += exp(static_cast<double>(logit_at(a, row, e)) - static_cast<double>(top));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    return sum == 0.0 ? 0.0 : 1.0 / sum;
+  }
+  __device__ __forceinline__ double value(int e, double by) const {
+    const double x = static_cast<double>(logit_at(a, row, e));
+    const double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - static_cast<double>(top)) * by;
+    return a.bias != nullptr ? s + static_cast<double>(a.bias[e]) : s;
+  }
+};
 
 // The choice of one token among the values c of its lanes' experts: lane j < top_k receives the j-th expert.  Exact, and the slow way:
 // up to 3000 instructions a token.
@@ -135,7 +163,7 @@ __device__ __noinline__ int select_exact(const RouteArgs& a, const V (&c)[P], V*
 // 2 kOff + kCut of one another), or kOpen (too close for that, or equal with low bits lost: select_exact has to choose).
 enum Selected { kFound, kOrder, kOpen };
 template <int P, bool kMargin>
-__device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float (&c)[P], bool lossless, int& mine) {
+__device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float (&c)[P], bool lossless, const Exact& exact, int& mine) {
   constexpr uint32_t kLow = P > 8 ? 15u : 7u;
   constexpr float kOff = P > 8 ? 0x1p-19f : 0x1.8p-20f, kCut = static_cast<float>(kLow) * 0x1p-23f, kApart = P > 8 ? 0x1.8p-18f : 0x1p-18f;
   static_assert(2.f * kOff + kCut < kApart, "see above");
@@ -192,6 +220,34 @@ __device__ __forceinline__ Selected select_fast(const RouteArgs& a, const float 
       const uint32_t lo = mine_kept ? order_key(score - off) : 0xffffffffu;
       const uint32_t hi = mine_kept || lane * P >= a.E ? 0u : order_key(score + (off + kCut * size));
       fine = __reduce_min_sync(0xffffffffu, lo) > __reduce_max_sync(0xffffffffu, hi);
+      if (!fine && __all_sync(0xffffffffu, P <= 2 || lane * P >= a.E || apart(value(key[P > 2 ? 1 : 0]), value(key[P > 2 ? 2 : 0])))) {
+        // Which two are a lane's best is plain: their sums in 64 bits, two scores to a lane instead of all.
+        const double by = exact.scale(), none = lowest<double>();
+        double hi2[2] = {none, none};
+#pragma unroll
+        for (int i = 0; i < (P > 1 ? 2 : 1); ++i)
+          if (lane * P < a.E) {
+            const double v = exact.value(e0 + static_cast<int>(kLow - (key[i] & kLow)), by);
+            if (v == v) hi2[i] = v;
+          }
+        double most = fmax(hi2[0], hi2[1]), next = fmin(hi2[0], hi2[1]);
+        for (int o = 1; o < lanes; o <<= 1) {
+          const double b = __shfl_xor_sync(0xffffffffu, most, o), s = __shfl_xor_sync(0xffffffffu, next, o);
+          next = fmax(fmin(most, b), fmax(next, s));
+          most = fmax(most, b);
+        }
+        uint64_t left = lane * P < a.E ? order_key(a.top == 2 ? most + next : most) : 0ull;
+        mine_kept = false;
+        for (int j = 0; j < a.kept; ++j) {
+          const uint64_t first = warp_max(left);
+          const int who = __ffs(__ballot_sync(0xffffffffu, left == first)) - 1;
+          if ((lane ^ who) < lanes) {
+            mine_kept = true;
+            left = 0ull;
+          }
+        }
+        fine = true;
+      }
     } else {
       fine = lossless || last != __reduce_max_sync(0xffffffffu, open);
     }
@@ -272,10 +328,6 @@ __device__ __forceinline__ void load_row(const void* row, bool f32, bool vec, in
     if (e0 + i < E) v[i] = f32 ? static_cast<const float*>(row)[e0 + i] : bf16_bits_to_f32(static_cast<const uint16_t*>(row)[e0 + i]);
 }
 
-__device__ __forceinline__ float logit_at(const RouteArgs& a, const uint8_t* row, int e) {
-  return a.f32 ? reinterpret_cast<const float*>(row)[e] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[e]);
-}
-
 // One token: lane j < top_k returns its j-th choice and weight.  kScores: the choice is on c, else on the logits.
 template <int P, bool kScores>
 __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratch, int& my_expert, float& my_weight) {
@@ -301,8 +353,9 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
   }
+  const Exact exact{a, row, top};
   if (!kScores) {
-    if (!a.regular || select_fast<P, false>(a, l, a.f32 == 0, my_expert) != kFound) my_expert = select_exact<P, float>(a, l, reinterpret_cast<float*>(scratch));
+    if (!a.regular || select_fast<P, false>(a, l, a.f32 == 0, exact, my_expert) != kFound) my_expert = select_exact<P, float>(a, l, reinterpret_cast<float*>(scratch));
   } else {
     Selected found = kOpen;
     if (a.regular) {
@@ -316,25 +369,14 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
       // (|e^x| (2 + 1.16 |x|) 2^-24, what __expf may be off, is largest at small x: 2^-22)
 #pragma unroll
       for (int i = 0; i < P; ++i) c[i] += a.sigmoid ? __fdividef(1.f, 1.f + __expf(-l[i])) : __expf(l[i] - top) * by;
-      found = select_fast<P, true>(a, c, false, my_expert);
+      found = select_fast<P, true>(a, c, false, exact, my_expert);
     }
     if (found != kFound) {
-      double sum = 0.0;
-      if (!a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < P; ++i) sum += exp(static_cast<double>(l[i]) - static_cast<double>(top));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      }
-      const double inv = a.sigmoid || sum == 0.0 ? 0.0 : 1.0 / sum;
-      auto score = [&](float x, int e) {
-        const double s = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - static_cast<double>(top)) * inv;
-        return a.bias != nullptr ? s + static_cast<double>(a.bias[e]) : s;
-      };
+      const double by = exact.scale();
       if (found == kOrder) {  // the candidates in 64 bits, each by the lane that holds it
         const int n = a.top_k + 1;
         uint64_t key = 0;
-        if (lane < n) key = order_key(score(logit_at(a, row, my_expert), my_expert));
+        if (lane < n) key = order_key(exact.value(my_expert, by));
         int rank = 0, sorted = 0;
         for (int i = 0; i < n; ++i) {
           const uint64_t k = __shfl_sync(0xffffffffu, key, i);
@@ -348,8 +390,8 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
         my_expert = sorted;
       } else {
         double d[P];
-#pragma unroll  // (else the logits lie in local memory from the start: 8192 tokens 25.3 us instead of 24.2)
-        for (int i = 0; i < P; ++i) d[i] = e0 + i < a.E ? score(l[i], e0 + i) : 0.0;
+#pragma unroll 1  // (the logits again from memory: indexed by a loop they would lie in local memory from the start, 8192 tokens 25.3 us instead of 24.2)
+        for (int i = 0; i < P; ++i) d[i] = e0 + i < a.E ? exact.value(e0 + i, by) : 0.0;
         my_expert = select_exact<P, double>(a, d, scratch);
       }
     }
@@ -552,9 +594,10 @@ static int32_t launch_choose(const RouteArgs& a, int blocks, cudaStream_t st) {
   return launch_choose<16, kScores>(a, blocks, st);
 }
 
-// Tokens of a block, a warp to each up to 32.  Few, so that few warps share an SM's issue slots (512 tokens of 256 experts: 12.5 us with 16 to a block,
-// 12.1 with 8; 64 in one block, tables included: 19, in blocks of 4: 7.6), and as few blocks as that leaves, since every block of the tables
-// adds up the counts of all and waits for the others' lines (512 tokens: 14.2 us with 4 to a block).
+// Tokens of a block, a warp to each up to 32.  Few, so that few warps share an SM's issue slots (64 tokens of 256 experts,
+// tables included, in one block: 19 us, in blocks of 4: 7.6), and as few blocks as that leaves, since every block of the tables
+// adds up the counts of all and waits for the others' lines (512 tokens: 2 us more
+// with 4 to a block than with 8).
 static int block_tokens(int M) {
   int n = kRouteFewTokens;
   while (n < 16 && (M + n - 1) / n > 64) n *= 2;
