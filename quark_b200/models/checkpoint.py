@@ -77,6 +77,12 @@ def _as_f32(entry) -> np.ndarray:
     return _cond.bf16_to_f32(_as_bf16(entry))
 
 
+def _wide(entry) -> np.ndarray:
+    """A float tensor that the model holds in f32, as wide as it is stored."""
+    tag, a = entry
+    return _cond.bf16_to_f32(np.asarray(a, np.uint16)) if tag == "BF16" else np.asarray(a, np.float32)
+
+
 def params_from_state_dict(raw: dict, cfg) -> dict:
     """Upstream-format state dict (``read_safetensors`` output) -> ``make_params``-layout host parameters."""
     d, ns = cfg.d_model, len(cfg.scheduler_sigmas)
@@ -134,6 +140,12 @@ def params_from_state_dict(raw: dict, cfg) -> dict:
                    "moe.expert_out": _as_bf16(need(p + moe_pre + "expert_out")).reshape(E * d, Hm)}  # fmt: skip
             if mlp["moe.router.weight"].shape != (E, d):
                 raise ValueError(f"block {i}: router weight is {mlp['moe.router.weight'].shape}, expected {(E, d)}")
+            if cfg.moe_score_bias:
+                mlp["moe.score_bias"] = _wide(need(p + moe_pre + "score_bias")).reshape(-1)
+                if mlp["moe.score_bias"].size != E:
+                    raise ValueError(f"block {i}: score bias has {mlp['moe.score_bias'].size} elements, expected {E}")
+            elif p + moe_pre + "score_bias" in raw:
+                raise ValueError(f"block {i}: the checkpoint's router has a score bias, the configuration says moe_score_bias=False")
         blk = {
             "qkv.weight": np.concatenate([_as_bf16(need(p + f"attn.{n}_proj.weight")) for n in ("q", "k", "v")], axis=0),
             "out.weight": _as_bf16(need(p + "attn.out_proj.weight")),

@@ -202,7 +202,8 @@ class Waypoint15Config:
     _YAML_SCALARS = ("d_model", "n_layers", "n_heads", "n_kv_heads", "mlp_ratio", "channels", "height", "width", "local_window",
                      "global_window", "global_pinned_dilation", "global_attn_period", "global_attn_offset", "value_residual",
                      "fourier_dim", "n_buttons", "ctrl_conditioning_period", "moe", "moe_n_experts", "moe_top_k", "moe_routing", "moe_scoring",
-                     "moe_n_groups", "moe_topk_groups", "moe_group_top", "moe_renormalize", "moe_route_scale", "moe_score_bias", "quilt_factor")  # fmt: skip
+                     "moe_n_groups", "moe_topk_groups", "moe_group_top", "moe_renormalize", "moe_route_scale", "moe_score_bias", "quilt_factor",
+                     "fp8_blocks")  # fmt: skip
 
     @classmethod
     def from_dict(cls, raw: dict, **overrides) -> "Waypoint15Config":
@@ -332,6 +333,16 @@ def shard_block_params(cfg: Waypoint15Config, blk: dict) -> dict:
 # ---------------------------------------------------------------------------
 # model
 # ---------------------------------------------------------------------------
+
+
+def score_bias_of(block: dict, n_experts: int) -> np.ndarray:
+    """The score bias among a block's host parameters, f32 ``[n_experts]``."""
+    if "moe.score_bias" not in block:
+        raise KeyError("the configuration says moe_score_bias, the block's parameters hold no score bias (moe.score_bias)")
+    b = np.ascontiguousarray(block["moe.score_bias"], dtype=np.float32).reshape(-1)
+    if b.size != n_experts:
+        raise ValueError(f"moe.score_bias has {b.size} elements for {n_experts} experts")
+    return b
 
 
 class TransformerBlock(nn.Module):
@@ -514,7 +525,7 @@ class Waypoint15(nn.Module):
                 blk.mlp.expert_in.data = up(p["moe.expert_in"])
                 blk.mlp.expert_out.data = up(p["moe.expert_out"])
                 if self.cfg.moe_score_bias:
-                    blk.mlp.score_bias.data = QuarkTensor.from_numpy(np.asarray(p["moe.score_bias"], dtype=np.float32))
+                    blk.mlp.score_bias.data = QuarkTensor.from_numpy(score_bias_of(p, self.cfg.moe_n_experts))
             else:
                 blk.mlp.fc1.weight.data = up(p["fc1.weight"])
                 blk.mlp.fc2.weight.data = up(p["fc2.weight"])

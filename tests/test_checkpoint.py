@@ -321,3 +321,62 @@ def test_moe_blocks_are_remapped(tmp_path):
         np.testing.assert_array_equal(blk["moe.router.weight"], sd[p + "router.weight"][1])
         np.testing.assert_array_equal(blk["moe.expert_in"].reshape(E, H, d)[3], sd[p + "expert_in"][1][3])
         np.testing.assert_array_equal(blk["moe.expert_out"].reshape(E, d, H)[5], trunc_bf16(sd[p + "expert_out"][1][5]))
+
+
+def scored_moe(cfg, seed=3):
+    """A checkpoint of routed experts, with a score bias in each block (stored f32, bf16 and 2-d in turn)."""
+    sd, r = synth_upstream(cfg), np.random.default_rng(seed)
+    E, H, d = cfg.moe_n_experts, cfg.mlp_dim // cfg.moe_top_k, cfg.d_model
+    for i in range(cfg.n_layers):
+        pre = f"transformer.blocks.{i}." + ("mlp." if i % 2 == 0 else "dit_mlp.")
+        del sd[pre + "fc1.weight"], sd[pre + "fc2.weight"]
+        for name, shape in (("router.weight", (E, d)), ("expert_in", (E, H, d)), ("expert_out", (E, d, H))):
+            sd[pre + name] = ("BF16", _cond._bf16(r.standard_normal(shape, dtype=np.float32)))
+        b = r.standard_normal(E).astype(np.float32)
+        sd[pre + "score_bias"] = ("BF16", _cond._bf16(b)) if i == 1 else ("F32", b.reshape(1, E) if i == 2 else b)
+    return sd
+
+
+SCORED = dict(moe=True, moe_n_experts=16, moe_top_k=2, moe_scoring="sigmoid", moe_n_groups=4, moe_topk_groups=2, moe_group_top=2, moe_route_scale=2.5)
+
+
+def test_score_biases_are_read(tmp_path):
+    """The bias of a router by scores is f32 and stays as wide as it is stored; ``Engine(model_uri)`` finds it under ``moe.score_bias``."""
+    from quark_b200.models import Waypoint15Config, make_params
+
+    cfg = tiny_cfg(**SCORED, moe_score_bias=True, ctrl_conditioning=False)
+    sd = scored_moe(cfg)
+    write_model_dir(cfg, tmp_path, extra_yaml="".join(f"{k}: {str(v).lower()}\n" for k, v in SCORED.items()) + "moe_score_bias: true\nfp8_blocks: true\n")
+    ck.write_safetensors(tmp_path / "model.safetensors", sd)
+    got = Waypoint15Config.from_yaml(tmp_path)
+    assert got.fp8_blocks and all(getattr(got, k) == v for k, v in SCORED.items()) and got.moe_score_bias
+    for i, (blk, ref) in enumerate(zip(ck.load_checkpoint(tmp_path, got)["blocks"], make_params(cfg)["blocks"])):
+        entry = sd[f"transformer.blocks.{i}." + ("mlp." if i % 2 == 0 else "dit_mlp.") + "score_bias"]
+        want = w32(entry)[0] if entry[0] == "BF16" else entry[1]
+        b = blk["moe.score_bias"]
+        assert b.dtype == np.float32 and b.shape == (16,) and [k for k in sorted(blk) if "moe" in k] == [k for k in sorted(ref) if "moe" in k]
+        np.testing.assert_array_equal(b, want.reshape(-1))
+
+
+def test_score_biases_that_do_not_fit_the_configuration():
+    cfg = tiny_cfg(**SCORED, moe_score_bias=True)
+    sd, name = scored_moe(cfg), "transformer.blocks.3.dit_mlp.score_bias"
+    with pytest.raises(KeyError, match="blocks.3.dit_mlp.score_bias"):  # the configuration wants one
+        ck.params_from_state_dict({k: v for k, v in sd.items() if k != name}, cfg)
+    with pytest.raises(ValueError, match="score bias"):  # the file has one that the configuration would leave out
+        ck.params_from_state_dict(sd, tiny_cfg(**SCORED))
+    with pytest.raises(ValueError, match="score bias"):
+        ck.params_from_state_dict({**sd, name: ("F32", np.zeros(8, np.float32))}, cfg)
+
+
+def test_a_score_bias_that_is_missing_among_host_parameters():
+    from quark_b200.models import make_params
+    from quark_b200.models.waypoint_15 import score_bias_of
+
+    blk = make_params(tiny_cfg(**SCORED, moe_score_bias=True))["blocks"][0]
+    assert score_bias_of(blk, 16).shape == (16,)
+    with pytest.raises(ValueError, match="8 experts"):
+        score_bias_of(blk, 8)
+    del blk["moe.score_bias"]
+    with pytest.raises(KeyError, match="no score bias"):
+        score_bias_of(blk, 16)
