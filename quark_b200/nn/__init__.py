@@ -14,6 +14,7 @@ from collections import OrderedDict
 import numpy as np
 
 from .. import functional as qf
+from ..runtime import stream as _stream
 from ..runtime.tensor import QuarkTensor
 
 
@@ -139,6 +140,9 @@ class Linear(Module):
         if fp8 and not self._fp8_skip and not self._fp8:
             if fp8_blocks:
                 self.weight.data, self.w_blocks = qf.quantize_e4m3_blocks(self.weight.data, tile_rows=qf.BLOCK)
+                # That kernel lets the next ones begin early, and a product fetches weights before it waits (b_constant): it could be before
+                # they are written.  (The other two forms let nothing begin early.)
+                _stream.synchronize()
             elif fp8_scaled:
                 self.weight.data, self.w_scale = qf.quantize_e4m3_rows(self.weight.data)
             else:

@@ -1,0 +1,69 @@
+"""Layers with block-scaled weights on the host: what they launch, wait for and keep, with the device calls replaced by a record of them."""
+
+import pytest
+
+from quark_b200 import nn
+from quark_b200.runtime.tensor import QuarkTensor
+
+
+def t(*shape, dtype="bf16"):
+    """A tensor of made-up memory: nothing below reads it."""
+    return QuarkTensor.borrow(1 << 20, shape, dtype)
+
+
+class Record:
+    """In the place of ``qf`` and of the stream: every call by its name, results of the right kind."""
+
+    BLOCK = 128
+
+    def __init__(self):
+        self.calls = []
+
+    def synchronize(self):
+        self.calls.append("synchronize")
+
+    def quantize_e4m3(self, X, out=None):
+        self.calls.append("quantize_e4m3")
+        return t(*X.shape, dtype="e4m3")
+
+    def quantize_e4m3_rows(self, X):
+        self.calls.append("quantize_e4m3_rows")
+        return t(*X.shape, dtype="e4m3"), t(X.shape[0], dtype="f32")
+
+    def quantize_e4m3_blocks(self, X, tile_rows=1, out=None, scale_out=None):
+        self.calls.append(f"quantize_e4m3_blocks {tile_rows}")
+        rows = -(-X.shape[0] // tile_rows)
+        return t(*X.shape, dtype="e4m3"), t(*((rows, -(-X.shape[1] // 128)) if tile_rows > 1 else (-(-X.shape[1] // 128), rows)), dtype="f32")
+
+    def gemm(self, A, B, out_dtype=None, activation=None, out=None, **kw):
+        assert A.dtype in ("bf16", "e4m3") and (A.dtype == "bf16" or B.dtype == "e4m3")
+        self.calls.append(f"gemm {A.dtype} {B.dtype} -> {out_dtype}")
+        return t(A.shape[0], B.shape[0], dtype=out_dtype)
+
+    def gemm_blocks(self, A, B, a_scale, b_scale, out_dtype=None, out=None, scale_out=None, **kw):
+        assert A.dtype == B.dtype == "e4m3" and a_scale.dtype == b_scale.dtype == "f32"
+        self.calls.append(f"gemm_blocks -> {out_dtype}")
+        y = t(A.shape[0], B.shape[0], dtype=out_dtype)
+        return y if out_dtype != "e4m3" else (y, t(-(-B.shape[0] // 128), A.shape[0], dtype="f32"))
+
+    def silu(self, X, out=None, out_q=None):
+        self.calls.append("silu" if out_q is None else "silu e4m3")
+
+
+@pytest.fixture
+def record(monkeypatch):
+    r = Record()
+    monkeypatch.setattr(QuarkTensor, "zeros", staticmethod(t))
+    monkeypatch.setattr(QuarkTensor, "empty", staticmethod(t))
+    monkeypatch.setattr(nn, "qf", r)
+    monkeypatch.setattr(nn, "_stream", r, raising=False)
+    return r
+
+
+def test_a_narrowed_weight_is_in_place_before_the_first_product(record):
+    """Products fetch weights ahead of the kernels before them (``b_constant``): the kernel that writes the weight may not be one of those."""
+    lin = nn.Linear(256, 384)
+    lin.prepare(fp8=True, fp8_blocks=True)
+    assert record.calls == ["quantize_e4m3_blocks 128", "synchronize"]
+    lin.prepare(fp8=True, fp8_blocks=True)  # once only
+    assert len(record.calls) == 2

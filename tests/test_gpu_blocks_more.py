@@ -1,0 +1,45 @@
+"""Block-scaled e4m3 and routing by scores: calls that follow one another closely, products whose CTAs walk several tiles, choices among
+equal scores, weights of scores far apart.  Formulas and tolerances are those of ``test_gpu_blocks``."""
+
+import numpy as np
+import pytest
+
+from tests import util
+from tests.test_gpu_blocks import T
+from tests.util import bf16_randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def qb():
+    import quark_b200 as q
+
+    q._lib.require_device(0)
+    yield q
+    q.runtime.synchronize()
+    assert q._lib.device_status() == 0
+
+
+# --------------------------------------------------------------------------------------------------------------- layers
+
+
+def test_a_product_right_after_its_weight_was_narrowed(qb):
+    """Rows that were narrowed before: nothing but the product follows the kernel that writes the weight.  The bits are those of the same call later."""
+    from quark_b200 import nn
+
+    r = util.rng(30)
+    K, N = 8192, 8192
+    x, s = qb.qf.quantize_e4m3_blocks(T(qb, bf16_randn(r, (3, K)), "bf16"))
+    for seed in range(4):
+        lin = nn.Linear(K, N)
+        wide = T(qb, np.resize(bf16_randn(util.rng([31, seed]), (1_000_003,), 0.05), (N, K)), "bf16")
+        lin.weight.data = wide  # (kept: giving its memory back would wait for the kernel that reads it)
+        out = [qb.QuarkTensor.zeros(3, N) for _ in range(2)]
+        qb.runtime.synchronize()
+        lin.prepare(fp8=True, fp8_blocks=True)
+        lin((x, s), out=out[0])
+        qb.runtime.synchronize()
+        lin((x, s), out=out[1])
+        np.testing.assert_array_equal(out[0].to_numpy(), out[1].to_numpy())
+        assert np.any(out[1].to_numpy() != 0)
