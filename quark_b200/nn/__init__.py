@@ -157,6 +157,8 @@ class Linear(Module):
         such a pair."""
         if self.w_blocks is not None:
             return self._forward_blocks(x, activation, bias, gate, residual, gate_groups, out_dtype, out, tp_arena)
+        if isinstance(x, tuple):
+            raise TypeError("Linear: a pair (e4m3, scales) needs a block-scaled weight (call prepare(fp8=True, fp8_blocks=True))")
         a_dt = x.dtype
         if tp_arena is not None:
             if activation is not None or bias is not None or gate is not None or self._has_bias or self.w_scale is not None:
@@ -350,7 +352,8 @@ class MLP(Module):
 
     ``fuse_silu=True`` folds SiLU into fc1's epilogue (the reference does so on its PTX and Metal
     GEMMs, ``src/quark/kernels/gemm/spec.py:54-59``); otherwise SiLU is its own launch as on the
-    reference's cuBLAS route.  With an fp8 fc2 the hidden activation is handed over in e4m3.
+    reference's cuBLAS route.  With an fp8 fc2 the hidden activation is handed over in e4m3 (in bf16 where one of the two linears has
+    block scales and the other has not).
     """
 
     def __init__(self, d_in: int, d_mid: int, d_out: int, out_dtype: str = "bf16", *, hidden_out_dtype: str | None = None, fuse_silu: bool = False):
@@ -361,8 +364,10 @@ class MLP(Module):
 
     def forward(self, x, *, gate=None, residual=None, gate_groups: int = 1, out=None, tp_arena=None):
         fp8 = self.fc2.weight.data.dtype == "e4m3"
-        if self._fuse_silu:  # (block scales: an e4m3 result comes with its scales)
-            h = self.fc1(x, activation="silu", out_dtype="e4m3" if fp8 else None)
+        if self._fuse_silu:
+            # (an e4m3 result of block-scaled weights comes with its scales, another without: fc2 has to know the same form)
+            alike = (self.fc1.w_blocks is None) == (self.fc2.w_blocks is None)
+            h = self.fc1(x, activation="silu", out_dtype="e4m3" if fp8 and alike else None)
         elif self.fc2.w_blocks is not None:
             h = self.silu(self.fc1(x))
         else:

@@ -67,3 +67,40 @@ def test_a_narrowed_weight_is_in_place_before_the_first_product(record):
     assert record.calls == ["quantize_e4m3_blocks 128", "synchronize"]
     lin.prepare(fp8=True, fp8_blocks=True)  # once only
     assert len(record.calls) == 2
+
+
+FORMS = {"bf16": {}, "e4m3": dict(fp8=True), "rows": dict(fp8=True, fp8_scaled=True), "blocks": dict(fp8=True, fp8_blocks=True)}
+
+
+@pytest.mark.parametrize("first", list(FORMS))
+@pytest.mark.parametrize("second", list(FORMS))
+@pytest.mark.parametrize("fuse", [False, True])
+def test_the_two_linears_of_an_mlp_are_narrowed_each_as_it_likes(record, first, second, fuse):
+    """The hidden activations are handed over in a form that both know: e4m3 with its scales between two block-scaled linears, plain e4m3
+    where neither is, else bf16."""
+    mlp = nn.MLP(256, 512, 256, fuse_silu=fuse)
+    mlp.fc1.prepare(**FORMS[first])
+    mlp.fc2.prepare(**FORMS[second])
+    del record.calls[:]
+    y = mlp(t(5, 256))
+    assert y.dtype == "bf16" and y.shape == (5, 256)
+    h = "e4m3" if second != "bf16" and (first == "blocks") == (second == "blocks") else "bf16"
+    if fuse:
+        one = [f"gemm_blocks -> {h}"] if first == "blocks" else [f"gemm bf16 {'bf16' if first == 'bf16' else 'e4m3'} -> {h}"]
+    else:
+        emit = second in ("e4m3", "rows")
+        h = "e4m3" if emit else "bf16"
+        one = ["gemm_blocks -> bf16" if first == "blocks" else f"gemm bf16 {'bf16' if first == 'bf16' else 'e4m3'} -> bf16", "silu e4m3" if emit else "silu"]
+    narrow = ["quantize_e4m3_blocks 1"]
+    handed = fuse and h == "e4m3"
+    two = (([] if handed else narrow) + ["gemm_blocks -> bf16"]) if second == "blocks" else [f"gemm {h} {'bf16' if second == 'bf16' else 'e4m3'} -> bf16"]
+    assert record.calls == (narrow if first == "blocks" else []) + one + two
+
+
+def test_a_pair_goes_with_block_scaled_weights_only(record):
+    lin = nn.Linear(256, 128)
+    pair = (t(4, 256, dtype="e4m3"), t(2, 4, dtype="f32"))
+    for form in ("bf16", "e4m3"):
+        lin.prepare(**FORMS[form])
+        with pytest.raises(TypeError, match="pair"):
+            lin(pair)
