@@ -507,7 +507,7 @@ class Waypoint15(nn.Module):
 
     def load_params(self, params: dict) -> "Waypoint15":
         """Upload a ``make_params``-style dict (full-size weights; a tensor-parallel rank keeps its slices);
-        call ``prepare()`` afterwards."""
+        call ``prepare()`` afterwards, also where the model had been prepared before."""
         up = lambda a: QuarkTensor.from_numpy(np.asarray(a), dtype="bf16")  # noqa: E731
         self.patchify.weight.data = up(params["patchify.weight"])
         self.unpatchify.weight.data = up(params["unpatchify.weight"])
@@ -518,17 +518,16 @@ class Waypoint15(nn.Module):
             self.ctrl_emb.fc2.weight.data = up(params["ctrl_emb.fc2.weight"])
         for blk, p in zip(self.blocks, params["blocks"]):
             p = shard_block_params(self.cfg, p)
-            blk.qkv_proj.weight.data = up(p["qkv.weight"])
-            blk.out_proj.weight.data = up(p["out.weight"])
+            blk.qkv_proj.load_weight(up(p["qkv.weight"]))
+            blk.out_proj.load_weight(up(p["out.weight"]))
             if self.cfg.moe:
                 blk.mlp.router.weight.data = up(p["moe.router.weight"])
-                blk.mlp.expert_in.data = up(p["moe.expert_in"])
-                blk.mlp.expert_out.data = up(p["moe.expert_out"])
+                blk.mlp.load_experts(up(p["moe.expert_in"]), up(p["moe.expert_out"]))
                 if self.cfg.moe_score_bias:
                     blk.mlp.score_bias.data = QuarkTensor.from_numpy(score_bias_of(p, self.cfg.moe_n_experts))
             else:
-                blk.mlp.fc1.weight.data = up(p["fc1.weight"])
-                blk.mlp.fc2.weight.data = up(p["fc2.weight"])
+                blk.mlp.fc1.load_weight(up(p["fc1.weight"]))
+                blk.mlp.fc2.load_weight(up(p["fc2.weight"]))
             if hasattr(blk, "ctrl_fusion"):
                 blk.ctrl_fusion.fc1_x.weight.data = up(p["ctrl.fc1_x.weight"])
                 blk.ctrl_fusion.fc1_c.weight.data = up(p["ctrl.fc1_c.weight"])

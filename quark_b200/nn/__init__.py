@@ -131,6 +131,11 @@ class Linear(Module):
         if bias:
             self.bias = Parameter(QuarkTensor.zeros(out_features, dtype="bf16"))
 
+    def load_weight(self, data) -> None:
+        """A new bf16 weight; what ``prepare`` made of the last one goes, and the next ``prepare`` narrows this one."""
+        self.weight.data = data
+        self._fp8, self.w_scale, self.w_blocks = False, None, None
+
     def prepare(self, *, shuffle: bool = False, fp8: bool = False, fp8_scaled: bool = False, fp8_blocks: bool = False, **kwargs):
         """``fp8_scaled`` (extension): narrow with one scale per output channel (``amax / 448``) instead of unscaled;
         the scales stay with the layer and are applied in the GEMM's epilogue.  ``fp8_blocks`` (extension): narrow with one scale
@@ -262,6 +267,11 @@ class MoE(Module):
         self.expert_out = Parameter(QuarkTensor.zeros(n_experts * d_model, d_intermediate, dtype="bf16"))
         self._fp8 = False
         self._blocks = None  # the experts' scales after prepare(fp8_blocks=True)
+
+    def load_experts(self, expert_in, expert_out) -> None:
+        """New bf16 weights of the experts; what ``prepare`` made of the last ones goes, and the next ``prepare`` narrows these."""
+        self.expert_in.data, self.expert_out.data = expert_in, expert_out
+        self._fp8, self._blocks = False, None
 
     def prepare(self, *, fp8: bool = False, moe_fp8: bool | None = None, fp8_blocks: bool = False, **kwargs):
         use = fp8 if moe_fp8 is None else moe_fp8

@@ -104,3 +104,42 @@ def test_a_pair_goes_with_block_scaled_weights_only(record):
         lin.prepare(**FORMS[form])
         with pytest.raises(TypeError, match="pair"):
             lin(pair)
+
+
+@pytest.mark.parametrize("form", ["e4m3", "rows", "blocks"])
+def test_a_new_weight_is_narrowed_again(record, form):
+    lin = nn.Linear(256, 200)
+    lin.prepare(**FORMS[form])
+    lin.load_weight(t(200, 256))
+    assert lin.weight.data.dtype == "bf16" and lin.w_blocks is None and lin.w_scale is None and list(lin.state_dict()) == ["weight"]
+    lin(t(4, 256))
+    assert record.calls[-1] == "gemm bf16 bf16 -> bf16"
+    del record.calls[:]
+    lin.prepare(**FORMS[form])
+    assert lin.weight.data.dtype == "e4m3" and (lin.w_blocks is not None) == (form == "blocks") and (lin.w_scale is not None) == (form == "rows")
+
+
+def test_parameters_loaded_into_a_prepared_model(record, monkeypatch):
+    """``load_params`` takes a model back to bf16 weights, and ``prepare`` narrows them again."""
+    from quark_b200.models import QuantConfig, Waypoint15, Waypoint15Config, make_params
+    from quark_b200.models import waypoint_15 as w
+
+    monkeypatch.setattr(QuarkTensor, "from_numpy", staticmethod(lambda a, dtype=None: t(*a.shape, dtype=dtype or "f32")))
+    monkeypatch.setattr(w, "_stream", record)
+    for kw in (dict(), dict(moe=True, moe_n_experts=8, moe_top_k=2)):
+        cfg = Waypoint15Config(d_model=128, n_layers=2, n_heads=2, n_kv_heads=1, height=8, width=8, channels=4, local_window=2, global_window=4, global_pinned_dilation=2,
+                               fourier_dim=32, quant=QuantConfig.all_fp8(), fp8_blocks=True, **kw)  # fmt: skip
+        model, params = Waypoint15(cfg), make_params(cfg)
+
+        def forms(blk):
+            lins = [blk.qkv_proj, blk.out_proj, *(() if cfg.moe else (blk.mlp.fc1, blk.mlp.fc2))]
+            got = {(lin.weight.data.dtype, lin.w_blocks is not None) for lin in lins}
+            if cfg.moe:
+                got |= {(p.data.dtype, blk.mlp._blocks is not None) for p in (blk.mlp.expert_in, blk.mlp.expert_out)}
+            return got
+
+        for _ in range(2):
+            model.load_params(params)
+            assert all(forms(blk) == {("bf16", False)} for blk in model.blocks)
+            model.prepare()
+            assert all(forms(blk) == {("e4m3", True)} for blk in model.blocks)

@@ -43,3 +43,28 @@ def test_a_product_right_after_its_weight_was_narrowed(qb):
         lin((x, s), out=out[1])
         np.testing.assert_array_equal(out[0].to_numpy(), out[1].to_numpy())
         assert np.any(out[1].to_numpy() != 0)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(moe=True, moe_n_experts=8, moe_top_k=2)])
+def test_parameters_loaded_into_a_model_that_was_prepared(qb, kw):
+    """A second set of parameters, and then the first again: every frame is that of a session made with them."""
+    from quark_b200.models import QuantConfig, Waypoint15Config, make_params
+    from tests.test_gpu_model import small_cfg
+
+    quant = QuantConfig(linear="fp8", kv_cache="bf16", attn_compute="bf16", moe="fp8")
+    cfg = Waypoint15Config(**{**small_cfg(qb, "bf16").__dict__, "quant": quant, "fp8_blocks": True, **kw})
+    params = [make_params(cfg, seed=s, weight_std=0.04) for s in (32, 33)]
+    noise = util.rng(34).standard_normal((1, cfg.latent_numel)).astype(np.float32)
+    want, got = [], []
+    for p in params:
+        want.append(qb.Engine(cfg=cfg, quant=quant, params=p, use_graph=False).gen_frame(noise=noise).reshape(-1))
+    eng = qb.Engine(cfg=cfg, quant=quant, params=params[0], use_graph=False)
+    start = eng.snapshot()
+    for p in (params[1], params[0]):
+        eng.model.load_params(p)
+        eng.model.prepare()
+        eng.restore(start)
+        got.append(eng.gen_frame(noise=noise).reshape(-1))
+    np.testing.assert_array_equal(got[0], want[1])
+    np.testing.assert_array_equal(got[1], want[0])
+    assert np.any(want[0] != want[1])
