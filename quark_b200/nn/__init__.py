@@ -127,24 +127,31 @@ class Linear(Module):
         self._fp8_skip = fp8_skip
         self._fp8 = False
         self.w_scale = None  # f32 [out_features] after prepare(fp8=True, fp8_scaled=True)
-        self.w_blocks = None  # f32 [ceil(out_features / 128), ceil(in_features / 128)] after prepare(fp8=True, fp8_blocks=True)
+        self.weight_blocks = None  # after prepare(fp8=True, fp8_blocks=True) a Parameter: the weight's scales, f32 [ceil(out / 128), ceil(in / 128)]
         if bias:
             self.bias = Parameter(QuarkTensor.zeros(out_features, dtype="bf16"))
+
+    @property
+    def w_blocks(self):
+        """The scales of a block-scaled weight, None of another."""
+        return self.weight_blocks.data if self.weight_blocks is not None else None
 
     def load_weight(self, data) -> None:
         """A new bf16 weight; what ``prepare`` made of the last one goes, and the next ``prepare`` narrows this one."""
         self.weight.data = data
-        self._fp8, self.w_scale, self.w_blocks = False, None, None
+        self._fp8, self.w_scale, self.weight_blocks = False, None, None
 
     def prepare(self, *, shuffle: bool = False, fp8: bool = False, fp8_scaled: bool = False, fp8_blocks: bool = False, **kwargs):
         """``fp8_scaled`` (extension): narrow with one scale per output channel (``amax / 448``) instead of unscaled;
         the scales stay with the layer and are applied in the GEMM's epilogue.  ``fp8_blocks`` (extension): narrow with one scale
-        per 128 x 128 tile; the activations are then narrowed with one per row and 128 channels (``qf.gemm_blocks``)."""
+        per 128 x 128 tile, which become a parameter, ``weight_blocks``; the activations are then narrowed with one per row and 128
+        channels (``qf.gemm_blocks``)."""
         if shuffle:
             raise RuntimeError("weight shuffling is not supported (it is disabled upstream as well)")
         if fp8 and not self._fp8_skip and not self._fp8:
             if fp8_blocks:
-                self.weight.data, self.w_blocks = qf.quantize_e4m3_blocks(self.weight.data, tile_rows=qf.BLOCK)
+                self.weight.data, scales = qf.quantize_e4m3_blocks(self.weight.data, tile_rows=qf.BLOCK)
+                self.weight_blocks = Parameter(scales)
                 # That kernel lets the next ones begin early, and a product fetches weights before it waits (b_constant): it could be before
                 # they are written.  (The other two forms let nothing begin early.)
                 _stream.synchronize()
@@ -160,7 +167,7 @@ class Linear(Module):
 
         With block scales ``x`` may be a pair ``(e4m3, scales)`` as ``qf.quantize_e4m3_blocks`` returns it, and ``out_dtype="e4m3"`` returns
         such a pair."""
-        if self.w_blocks is not None:
+        if self.weight_blocks is not None:
             return self._forward_blocks(x, activation, bias, gate, residual, gate_groups, out_dtype, out, tp_arena)
         if isinstance(x, tuple):
             raise TypeError("Linear: a pair (e4m3, scales) needs a block-scaled weight (call prepare(fp8=True, fp8_blocks=True))")
@@ -232,7 +239,8 @@ class MoE(Module):
 
     Extensions: ``scoring`` (``"softmax"`` or ``"sigmoid"``) routes by ``qf.moe_route_scored`` on f32 logits, up to 512 experts, with its ``n_groups``,
     ``topk_groups``, ``group_top``, ``renormalize`` and ``route_scale`` (its ``factor``); ``score_bias`` gives the layer a parameter of that name, f32
-    ``[E]``, that takes part in the choice.  ``prepare(fp8_blocks=True)`` narrows the experts' weights with a scale per 128 x 128 tile and
+    ``[E]``, that takes part in the choice.  ``prepare(fp8_blocks=True)`` narrows the experts' weights with a scale per 128 x 128 tile (the parameters
+    ``expert_in_blocks`` and ``expert_out_blocks``) and
     the activations with one per row and 128 channels (``qf.gemm_grouped_blocks``); both widths are then multiples of 128."""
 
     def __init__(self, M: int, d_model: int, d_intermediate: int, n_experts: int, top_k: int, *, routing: str = "correct", out_dtype: str = "bf16",
@@ -266,22 +274,22 @@ class MoE(Module):
         self.expert_in = Parameter(QuarkTensor.zeros(n_experts * d_intermediate, d_model, dtype="bf16"))
         self.expert_out = Parameter(QuarkTensor.zeros(n_experts * d_model, d_intermediate, dtype="bf16"))
         self._fp8 = False
-        self._blocks = None  # the experts' scales after prepare(fp8_blocks=True)
+        self.expert_in_blocks = self.expert_out_blocks = None  # Parameters after prepare(fp8_blocks=True): the experts' scales
 
     def load_experts(self, expert_in, expert_out) -> None:
         """New bf16 weights of the experts; what ``prepare`` made of the last ones goes, and the next ``prepare`` narrows these."""
         self.expert_in.data, self.expert_out.data = expert_in, expert_out
-        self._fp8, self._blocks = False, None
+        self._fp8, self.expert_in_blocks, self.expert_out_blocks = False, None, None
 
     def prepare(self, *, fp8: bool = False, moe_fp8: bool | None = None, fp8_blocks: bool = False, **kwargs):
         use = fp8 if moe_fp8 is None else moe_fp8
         if use and fp8_blocks and not self._fp8:
             if self._schedule != "sorted" or self._D % qf.BLOCK or self._H % qf.BLOCK:
                 raise ValueError(f"MoE: block scales need the sorted schedule and widths that are multiples of 128, got {self._D} and {self._H}")
-            self._blocks = []
-            for p in (self.expert_in, self.expert_out):  # (every expert has whole tiles of its own)
-                p.data, scale = qf.quantize_e4m3_blocks(p.data, tile_rows=qf.BLOCK)
-                self._blocks.append(scale)
+            # (every expert has whole tiles of its own)
+            self.expert_in.data, s_in = qf.quantize_e4m3_blocks(self.expert_in.data, tile_rows=qf.BLOCK)
+            self.expert_out.data, s_out = qf.quantize_e4m3_blocks(self.expert_out.data, tile_rows=qf.BLOCK)
+            self.expert_in_blocks, self.expert_out_blocks = Parameter(s_in), Parameter(s_out)
             self._fp8 = True
         elif use and not self._fp8:
             self.expert_in.data = qf.quantize_e4m3(self.expert_in.data)
@@ -292,7 +300,7 @@ class MoE(Module):
         M, D, H, E = x.numel // int(x.shape[-1]), self._D, self._H, self._E
         cd = "e4m3" if self._fp8 else None
         logits = self.router(x)
-        if self._scoring or self._blocks:
+        if self._scoring or self.expert_in_blocks is not None:
             return self._forward_scored(x, logits, M)
         if self._schedule == "sorted":
             n = qf.moe_slots(M, E, self._K)
@@ -335,11 +343,11 @@ class MoE(Module):
         bias = self.score_bias.data if hasattr(self, "score_bias") else None
         r = qf.moe_route_scored(logits, bias, top_k=K, out=[_cached(self, *t) for t in shapes], **self._route)
         partials = _cached(self, "partials_s", (n, D), "f32")
-        if self._blocks:
+        if self.expert_in_blocks is not None:
             xs = qf.quantize_e4m3_blocks(x, row_index=r.slot_token, out=_cached(self, "xs", (n, D), "e4m3"), scale_out=_cached(self, "xs_s", (D // qf.BLOCK, n), "f32"))
-            h = qf.gemm_grouped_blocks(xs[0], self.expert_in.data, xs[1], self._blocks[0], r.tile_expert, r.tile_rows, n_experts=E, activation="silu",
+            h = qf.gemm_grouped_blocks(xs[0], self.expert_in.data, xs[1], self.expert_in_blocks.data, r.tile_expert, r.tile_rows, n_experts=E, activation="silu",
                                        out=_cached(self, "h_s", (n, H), "e4m3"), scale_out=_cached(self, "h_ss", (H // qf.BLOCK, n), "f32"), b_constant=True)  # fmt: skip
-            qf.gemm_grouped_blocks(h[0], self.expert_out.data, h[1], self._blocks[1], r.tile_expert, r.tile_rows, n_experts=E, out=partials, b_constant=True)
+            qf.gemm_grouped_blocks(h[0], self.expert_out.data, h[1], self.expert_out_blocks.data, r.tile_expert, r.tile_rows, n_experts=E, out=partials, b_constant=True)
         else:
             od, cd = ("e4m3", "e4m3") if self._fp8 else ("bf16", None)
             xs = qf.moe_gather(x, r.slot_token, out=_cached(self, "xs", (n, D), od))

@@ -106,6 +106,27 @@ def test_a_pair_goes_with_block_scaled_weights_only(record):
             lin(pair)
 
 
+def test_scales_are_part_of_the_state(record):
+    """The e4m3 bytes mean nothing without their scales: both are in ``state_dict``, and a state goes only into layers narrowed the same way."""
+    a, b, plain = nn.Linear(256, 200), nn.Linear(256, 200), nn.Linear(256, 200)
+    for lin in (a, b):
+        lin.prepare(fp8=True, fp8_blocks=True)
+    state = a.state_dict()
+    assert list(state) == ["weight", "weight_blocks"] and state["weight_blocks"] is a.w_blocks and a.w_blocks.shape == (2, 2)
+    b.load_state_dict(state)
+    assert b.weight.data is a.weight.data and b.w_blocks is a.w_blocks
+    with pytest.raises(KeyError, match="weight_blocks"):
+        plain.load_state_dict(state)
+    with pytest.raises(KeyError, match="weight_blocks"):
+        b.load_state_dict(plain.state_dict())
+    moe, other = nn.MoE(4, 128, 256, 8, 2), nn.MoE(4, 128, 256, 8, 2)
+    moe.prepare(fp8=True, fp8_blocks=True)
+    state = moe.state_dict()
+    assert state["expert_in_blocks"].shape == (8 * 2, 1) and state["expert_out_blocks"].shape == (8 * 1, 2)
+    with pytest.raises(KeyError, match="expert_in_blocks"):
+        other.load_state_dict(state)
+
+
 @pytest.mark.parametrize("form", ["e4m3", "rows", "blocks"])
 def test_a_new_weight_is_narrowed_again(record, form):
     lin = nn.Linear(256, 200)
@@ -135,7 +156,7 @@ def test_parameters_loaded_into_a_prepared_model(record, monkeypatch):
             lins = [blk.qkv_proj, blk.out_proj, *(() if cfg.moe else (blk.mlp.fc1, blk.mlp.fc2))]
             got = {(lin.weight.data.dtype, lin.w_blocks is not None) for lin in lins}
             if cfg.moe:
-                got |= {(p.data.dtype, blk.mlp._blocks is not None) for p in (blk.mlp.expert_in, blk.mlp.expert_out)}
+                got |= {(p.data.dtype, "expert_in_blocks" in blk.mlp.state_dict()) for p in (blk.mlp.expert_in, blk.mlp.expert_out)}
             return got
 
         for _ in range(2):
