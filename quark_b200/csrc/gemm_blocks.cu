@@ -59,7 +59,7 @@ struct BlockSmem {
   static constexpr int kColOffset = kBarOffset + 256;  // per-column scale (unused), bias, gate
   static constexpr int kTopOffset = kColOffset + 3 * BN * 4;
   static constexpr int kTotal = kTopOffset + kColGroups * kBM * 4 + 1024;  // + alignment slack
-  static_assert((2 * kStages + kAccBuffers) * 8 + 32 <= 256 && kTotal <= 227 * 1024, "shared memory of one CTA");
+  static_assert((2 * kStages + kAccBuffers + 1) * 8 + 32 <= 256 && kTotal <= 227 * 1024, "shared memory of one CTA");
 };
 
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
@@ -98,7 +98,8 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   uint64_t* empty_bar = full_bar + kStages;
   static_assert(kStages >= kAccBuffers, "see above");
   uint64_t* acc_empty = empty_bar + kStages;      // [buffer] the warps that sum have read a block's products
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccBuffers);
+  uint64_t* drain_bar = acc_empty + kAccBuffers;  // the MMAs in flight when the CTA gives up are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* drain_flag = abort_flag + 1;  // never set: lets the drain waits below run their own limit
   volatile int* lost_flag = abort_flag + 2;   // set by a CTA of the cluster whose slice is missing
@@ -146,6 +147,7 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int b = 0; b < kAccBuffers; ++b) mbar_init(smem_u32(&acc_empty[b]), kSumWarps);
+    mbar_init(smem_u32(drain_bar), 1);
     *abort_flag = 0;
     *drain_flag = 0;
     *lost_flag = 0;
@@ -203,17 +205,23 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (++s == kStages) { s = 0; ph ^= 1; }
         }
       }
+      // s is the stage that was filled longest ago, and ph the parity of what it waits for, be it the end of the fill or its release; one
+      // that was never filled passes at once.
       if (alive && *abort_flag == 0) {
-        // Tail: see the last stage releases land before the CTA can exit (a stage that was never used passes at once).
+        // Tail: see the last stage releases land before the CTA can exit.
+        int ts = s;
+        uint32_t tph = ph;
         for (int i = 0; i < kStages; ++i) {
-          if (!mbar_wait(empty0 + s * 8, ph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
-          if (++s == kStages) { s = 0; ph ^= 1; }
+          if (!mbar_wait(empty0 + ts * 8, tph, abort_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM)) break;
+          if (++ts == kStages) { ts = 0; tph ^= 1; }
         }
       }
       if (*abort_flag) {
-        // Giving up: leave the copies already in flight time to land before this CTA's memory goes away.
-        const long long t0 = clock64();
-        while (clock64() - t0 < (1ll << 22)) __nanosleep(1000);
+        // Giving up: let the copies already in flight land before this CTA's memory goes away.
+        for (int i = 0; i < kStages; ++i) {
+          mbar_wait(full0 + s * 8, ph, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
+          if (++s == kStages) { s = 0; ph ^= 1; }
+        }
       }
     }
   } else if (warp == 1) {
@@ -255,6 +263,10 @@ gemm_blocks_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             umma_commit(release);
           }
         }
+      }
+      if (!alive || *abort_flag) {  // giving up: the MMAs in flight still read the stages and write TMEM
+        umma_commit(smem_u32(drain_bar));
+        mbar_wait(smem_u32(drain_bar), 0, drain_flag, g.status, QB_DEV_WAIT_TIMEOUT_GEMM);
       }
     }
   } else if (warp >= kW0) {
