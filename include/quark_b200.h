@@ -451,7 +451,7 @@ int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scal
  * 0 (a row without any finite logit).  NaN is chosen last and reaches the weights.  E <= 512, n_groups <= 32, top_k <= 32.
  * The slot tables (all or none of the five pointers), for n = qb_moe_scored_slots(M, E, top_k) slots, a multiple of 128 that any
  * routing fits: slot_token, slot_weight, tile_expert, token_slot as in qb_moe_route_slots, and tile_rows [n / 128], the slots of each
- * tile that hold a token (0 past the last used tile).  Workspace (may be NULL without tables and where its size is 0): the first 64 KiB
+ * tile that hold a token (0 past the last used tile); with them M <= 2^24.  Workspace (may be NULL without tables and where its size is 0): the first 64 KiB
  * are not touched, so that the workspace of qb_gemm can be lent; calls that share one must not overlap. */
 typedef struct {
   int32_t M, E, top_k;

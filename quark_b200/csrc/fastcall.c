@@ -466,7 +466,7 @@ static PyObject* fast_route_scored(PyObject* self, PyObject* const* a, Py_ssize_
   static const int dtypes[7] = {QB_S32, QB_F32, QB_S32, QB_F32, QB_S32, QB_S32, QB_S32};
   const Py_ssize_t want = tables ? 7 : 2;
   PyObject* const seq = a[10];
-  if (slots == 0 || PySequence_Fast_GET_SIZE(seq) != want) Py_RETURN_NONE;
+  if (slots == 0 || (tables && M > (1 << 24)) || PySequence_Fast_GET_SIZE(seq) != want) Py_RETURN_NONE;
   memset(o, 0, sizeof(o));
   for (Py_ssize_t i = 0; i < want; ++i)
     if (!tensor(PySequence_Fast_GET_ITEM(seq, i), &o[i]) || o[i].numel != numel[i] || o[i].dtype != dtypes[i]) Py_RETURN_NONE;

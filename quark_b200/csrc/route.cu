@@ -26,6 +26,9 @@ namespace qb {
 constexpr int kRouteMaxExperts = 512, kRouteMaxGroups = 32, kRouteMaxTopK = 32;
 constexpr int kRouteTokens = 64, kRouteFewTokens = 4;  // most and fewest tokens of a block
 constexpr int kRouteThreads = 1024;
+// Tokens of a call with tables.  Every block reads the counts of all, 64 tokens each: 14 ms at 2^20 tokens of 256 experts, some seconds here, and
+// the threads of all blocks, which slots are numbered by, stay far inside 32 bits.
+constexpr int kRouteMaxTableTokens = 1 << 24;
 constexpr int kRouteTile = 128;     // row tile of the grouped product
 constexpr size_t kRouteWsOffset = 64u << 10;  // the area in front belongs to the GEMM's counters
 
@@ -647,6 +650,7 @@ extern "C" int32_t qb_moe_route_scored(const void* logits, const float* bias, in
   const bool tables = slot_token != nullptr;
   QB_REQUIRE((slot_weight != nullptr) == tables && (tile_expert != nullptr) == tables && (tile_rows != nullptr) == tables && (token_slot != nullptr) == tables,
              QB_ERR_INVALID_ARG, "moe_route_scored: the slot tables come together");
+  QB_REQUIRE(!tables || p->M <= kRouteMaxTableTokens, QB_ERR_UNSUPPORTED, "moe_route_scored: slot tables of at most %d tokens (got %d)", kRouteMaxTableTokens, p->M);
   const uintptr_t all = reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(experts) | reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(slot_token) |
                         reinterpret_cast<uintptr_t>(slot_weight) | reinterpret_cast<uintptr_t>(tile_expert) | reinterpret_cast<uintptr_t>(tile_rows) |
                         reinterpret_cast<uintptr_t>(token_slot);

@@ -1150,6 +1150,8 @@ def moe_route_scored(logits, bias=None, *, top_k: int, scoring: str = "softmax",
     n = moe_scored_slots(M, E, k)
     if n == 0 or k > 32 or E > 512:
         raise ValueError(f"{who}: top_k {k} of {E} experts for {M} tokens (at most 32 of 512)")
+    if tables and M > 1 << 24:
+        raise ValueError(f"{who}: slot tables of at most {1 << 24} tokens (got {M}); route them in parts or without tables")
     if not (1 <= n_groups <= 32) or E % n_groups or not (1 <= topk_groups <= n_groups) or topk_groups * (E // n_groups) < k:
         raise ValueError(f"{who}: {topk_groups} of {n_groups} groups (at most 32) of {E} experts for top_k {k}")
     if group_top not in (1, 2) or (n_groups > 1 and E // n_groups < group_top):

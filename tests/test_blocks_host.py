@@ -123,3 +123,25 @@ def test_sizes_of_the_slot_tables():
 def test_python_checks(kind, call):
     with pytest.raises(kind):
         call()
+
+
+def test_tables_of_more_tokens_than_a_call_can_number(monkeypatch):
+    """Every block of the tables reads the counts of all: what 2^24 tokens leave is seconds of work, and past 2^28 the slots were numbered in too few bits."""
+    lib = _lib.load()
+
+    def route(tabs, **kw):
+        p = _lib.RouteParams(**{**dict(M=(1 << 24) + 1, E=8, top_k=1, logits_dtype=0, scoring=0, n_groups=1, topk_groups=1, group_top=1, renormalize=1, factor=1.0), **kw})
+        return lib.qb_moe_route_scored(ONE, None, ONE, ONE, *tabs, C.byref(p), ONE, 1 << 40, None)
+
+    assert route((ONE,) * 5) == -2 and "16777216 tokens" in last()
+    assert route((ONE,) * 5, M=1 << 28) == -2
+    assert route((None,) * 5, M=1 << 30) == -1  # (without tables only the size of the result counts)
+    big = t((1 << 24) + 1, 8)
+    with pytest.raises(ValueError, match="16777216 tokens"):
+        qf.moe_route_scored(big, top_k=1)
+    n = qf.moe_scored_slots((1 << 24) + 1, 8, 1)
+    out = [t(*s, dtype=d) for s, d in ((((1 << 24) + 1, 1), "s32"), (((1 << 24) + 1, 1), "f32"), ((n,), "s32"), ((n,), "f32"), ((n // 128,), "s32"), ((n // 128,), "s32"),
+                                       (((1 << 24) + 1, 1), "s32"))]  # fmt: skip
+    monkeypatch.setattr(qf, "_s", lambda: 1 << 20)
+    with pytest.raises(ValueError, match="16777216 tokens"):
+        qf.moe_route_scored(big, top_k=1, out=out)
