@@ -139,6 +139,8 @@ extern "C" int32_t qb_quantize_e4m3_blocks(const void* X, const int32_t* row_ind
   QB_REQUIRE(p != nullptr, QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: params are NULL");
   QB_REQUIRE(X && out && scale_out, QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: NULL pointer");
   QB_REQUIRE(p->batch > 0 && p->rows > 0 && p->cols > 0, QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: %d matrices of %d x %d", p->batch, p->rows, p->cols);
+  constexpr int kMost = 0x7fffffff - 127;  // rounded up to whole blocks it is still an int
+  QB_REQUIRE(p->cols <= kMost && (p->tile_rows == 1 || p->rows <= kMost), QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: %d x %d is too large", p->rows, p->cols);
   QB_REQUIRE(p->cols % 16 == 0, QB_ERR_ALIGN, "quantize_e4m3_blocks: %d columns (must be a multiple of 16)", p->cols);
   QB_REQUIRE(p->src_dtype == QB_BF16 || p->src_dtype == QB_F32, QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: source dtype %d", p->src_dtype);
   QB_REQUIRE(p->tile_rows == 1 || p->tile_rows == 128, QB_ERR_INVALID_ARG, "quantize_e4m3_blocks: tile_rows %d (1 or 128)", p->tile_rows);

@@ -637,6 +637,8 @@ static int32_t launch_blocks(const CUtensorMap& tmA, const CUtensorMap& tmA_smal
 static int32_t validate_blocks(const qb_gemm_blocks_params* p) {
   QB_REQUIRE(p != nullptr, QB_ERR_INVALID_ARG, "gemm_blocks: params are NULL");
   QB_REQUIRE(p->M > 0 && p->N > 0 && p->K > 0, QB_ERR_INVALID_ARG, "gemm_blocks: M, N, K must be positive (got %d, %d, %d)", p->M, p->N, p->K);
+  constexpr int kMost = 0x7fffffff - 255;  // rounded up to whole tiles it is still an int
+  QB_REQUIRE(p->M <= kMost && p->N <= kMost && p->K <= kMost, QB_ERR_INVALID_ARG, "gemm_blocks: M, N, K too large (got %d, %d, %d)", p->M, p->N, p->K);
   QB_REQUIRE(p->c_dtype == QB_BF16 || p->c_dtype == QB_F32 || p->c_dtype == QB_E4M3, QB_ERR_INVALID_ARG, "gemm_blocks: c_dtype %d", p->c_dtype);
   QB_REQUIRE(p->K % 16 == 0, QB_ERR_ALIGN, "gemm_blocks: K = %d must be a multiple of 16", p->K);
   QB_REQUIRE(p->N % 8 == 0, QB_ERR_ALIGN, "gemm_blocks: N = %d must be a multiple of 8", p->N);

@@ -145,3 +145,21 @@ def test_tables_of_more_tokens_than_a_call_can_number(monkeypatch):
     monkeypatch.setattr(qf, "_s", lambda: 1 << 20)
     with pytest.raises(ValueError, match="16777216 tokens"):
         qf.moe_route_scored(big, top_k=1, out=out)
+
+
+def test_sizes_next_to_the_largest_number_are_refused():
+    """The number of blocks and tiles of such a size left 32 bits: a contraction of 2^31 - 16 had a negative number of blocks in the kernel."""
+    lib, top = _lib.load(), (1 << 31) - 16
+
+    def gemm(**kw):
+        p = _lib.GemmBlocksParams(**{**dict(M=16, N=16, K=32, c_dtype=0, activation=0, gate_groups=1), **kw})
+        return lib.qb_gemm_blocks(ONE, ONE, ONE, ONE, ONE, None, None, None, None, C.byref(p), None)
+
+    def quant(**kw):
+        p = _lib.QuantBlocksParams(**{**dict(batch=1, rows=1, cols=32, src_rows=1, src_dtype=0, tile_rows=1, pow2=0), **kw})
+        return lib.qb_quantize_e4m3_blocks(ONE, None, ONE, ONE, C.byref(p), None)
+
+    for kw in (dict(M=top), dict(N=top), dict(K=top)):
+        assert gemm(**kw) == -1 and "too large" in last(), kw
+    for kw in (dict(cols=top), dict(rows=top, src_rows=top, tile_rows=128), dict(cols=top, tile_rows=128)):
+        assert quant(**kw) == -1 and "too large" in last(), kw
