@@ -415,7 +415,9 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
     by = s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) by += __shfl_xor_sync(0xffffffffu, by, o);
-    if (by < 1e-25f) {  // the bias chose experts whose scores leave 32 bits; their ratios do not
+    // The bias chose experts whose scores leave 32 bits (a subnormal one has lost bits, a sum this small may be of such); their ratios do not.
+    const bool tiny = lane < a.top_k && s < 1.17549435e-38f && x > __uint_as_float(0xff800000u);
+    if (by < 1e-25f || __any_sync(0xffffffffu, tiny)) {
       const double t = static_cast<double>(top);
       const double wide = lane < a.top_k ? (a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - t)) : 0.0;
       double all = wide;

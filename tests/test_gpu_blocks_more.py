@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from tests import util
-from tests.test_gpu_blocks import T
+from tests.test_gpu_blocks import T, check_routing, route
 from tests.util import bf16_randn
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,29 @@ def test_parameters_loaded_into_a_model_that_was_prepared(qb, kw):
     np.testing.assert_array_equal(got[0], want[1])
     np.testing.assert_array_equal(got[1], want[0])
     assert np.any(want[0] != want[1])
+
+
+# -------------------------------------------------------------------------------------------------------------- routing
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("low", [-70.0, -90.0, -95.0, -105.0, -120.0])
+def test_weights_of_choices_on_both_sides_of_what_32_bits_hold(qb, scoring, low):
+    """The bias picks experts of which some score far above the others: the small ones' weights are as close as the large ones', also where their
+    scores are subnormal or 0 in 32 bits and the sum is not small."""
+    r = util.rng([35, int(-low)])
+    x = r.standard_normal((70, 64)).astype(np.float32)
+    x[:, ::7] += np.float32(low)
+    x[:, 7] += np.float32(0.5 * -low)  # one of the ten is about halfway
+    bias = np.zeros(64, np.float32)
+    bias[::7] = 2.0 + np.arange(10)
+    for k in (2, 4, 10):
+        got = qb.qf.moe_route_scored(T(qb, x), T(qb, bias), top_k=k, scoring=scoring, factor=2.5)
+        e, w = route(x, bias, k, scoring, factor=2.5)
+        check_routing(got, e, w, 64)
+    masked = x.copy()
+    masked[:, 14] = -np.inf  # chosen by its bias all the same, with weight 0
+    got = qb.qf.moe_route_scored(T(qb, masked), T(qb, bias), top_k=10, scoring=scoring)
+    e, w = route(masked, bias, 10, scoring)
+    assert np.all((e == 14).sum(1) == 1) and np.all(w[e == 14] == 0)
+    check_routing(got, e, w, 64)
