@@ -4,8 +4,9 @@ equal scores, weights of scores far apart.  Formulas and tolerances are those of
 import numpy as np
 import pytest
 
+from oracle import codec
 from tests import util
-from tests.test_gpu_blocks import T, check_routing, route
+from tests.test_gpu_blocks import Operands, T, blocks, check, check_routing, epilogue, route, route_scores, values
 from tests.util import bf16_randn
 
 pytestmark = pytest.mark.gpu
@@ -94,3 +95,114 @@ def test_weights_of_choices_on_both_sides_of_what_32_bits_hold(qb, scoring, low)
     e, w = route(masked, bias, 10, scoring)
     assert np.all((e == 14).sum(1) == 1) and np.all(w[e == 14] == 0)
     check_routing(got, e, w, 64)
+
+
+def choice(values, groups, kept, top, k):
+    """The kept groups by the sum of their best ``top`` values, then the best ``k`` inside them; equal ones: the lower index."""
+    M, E = values.shape
+    per = -np.sort(-values.reshape(M, groups, -1), 2)[:, :, :top].sum(2)
+    keep = np.zeros((M, groups), bool)
+    np.put_along_axis(keep, np.argsort(-per, 1, kind="stable")[:, :kept], True, 1)
+    out = np.zeros((M, k), int)
+    for m in range(M):
+        inside = np.flatnonzero(np.repeat(keep[m], E // groups))
+        out[m] = inside[np.argsort(-values[m, inside], kind="stable")[:k]]
+    return out
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,kept,k", [(32, 4, 2, 6), (32, 8, 3, 12), (256, 8, 4, 8), (24, 4, 3, 5), (160, 8, 3, 6), (512, 16, 5, 32)])
+@pytest.mark.parametrize("top", [1, 2])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_equal_groups_and_experts_without_a_bias(qb, scoring, E, groups, kept, k, top, dtype):
+    """Every expert of every token, equal or masked, is the one the formula names: by the logits where groups go by their best one (-inf comes
+    behind the lowest value), by the scores in 64 bits where they go by their best two."""
+    r = util.rng([36, E, groups])
+    M, low = 150, codec.bf16_to_f32(np.uint16(0xFF7F)) if dtype == "bf16" else np.float32(-3.4028235e38)
+    # (no two levels are opposite: the sigmoids of such sum to 1 but for a rounding, and 64 bits would not say which group comes first)
+    x = r.integers(-2, 3, (M, E)).astype(np.float32) * np.float32(0.5) + np.float32(0.3125)
+    x[3:40] = np.where(r.random((37, E)) < 0.7, -np.inf, x[3:40])
+    x[40:70] = np.where(r.random((30, E)) < 0.7, low, x[40:70])
+    x[5], x[6], x[7] = -np.inf, 0.0, low
+    x[8, :] = np.where(np.arange(E) % 3 == 0, -np.inf, low)
+    x[9] = np.where(np.arange(E) < E // groups, 1.0, x[9])
+    x[70:80, ::2] = -0.0
+    x[70:80, 1::2] = 0.0
+    X = T(qb, codec.f32_to_bf16(x), "bf16") if dtype == "bf16" else T(qb, x)
+    got = qb.qf.moe_route_scored(X, top_k=k, scoring=scoring, n_groups=groups, topk_groups=kept, group_top=top)
+    s = route_scores(x, scoring)
+    e = choice(x.astype(np.float64) if top == 1 else s, groups, kept, top, k)
+    w = np.take_along_axis(s, e, 1)
+    t = w.sum(1, keepdims=True)
+    check_routing(got, e, np.where(t == 0, 0, w / np.where(t == 0, 1, t)), E)
+
+
+# ------------------------------------------------------------------------------------------------- several tiles to a CTA
+
+
+@pytest.mark.parametrize("tile_n,M,N,K", [
+    (64, 1700, 1400, 640), (64, 2000, 1096, 1152), (64, 2100, 1048, 144),
+    (128, 2500, 2056, 640), (128, 2700, 1880, 1152), (128, 2500, 2000, 272), (128, 2500, 2000, 1024),
+    (256, 2500, 4104, 640), (256, 2600, 3848, 384), (256, 2500, 4000, 128), (256, 2500, 4000, 1168),
+])  # fmt: skip
+@pytest.mark.parametrize("kind", ["plain", "bias_silu", "gate", "bias_silu_gate_groups"])
+def test_several_tiles_of_a_cta(qb, tile_n, M, N, K, kind):
+    """More tiles than SMs: a CTA's next tile meets the ring, the accumulators' buffers and the vectors per column as the last one left them.
+    Blocks of K that go evenly into the buffers and ones that do not, with every epilogue and type that the width has."""
+    tiles = -(-M // 128) * -(-N // tile_n)
+    assert tiles > 2 * 148 or tile_n == 64 and tiles > 148
+    r = util.rng([37, M, N, K])
+    op = Operands(r, M, N, K)
+    t = op.tensors(qb)
+    y, mags = op.product()
+    kw, ref = {}, {}
+    if "bias" in kind:
+        ref["bias"] = bf16_randn(r, (N,))
+        kw["bias"] = T(qb, ref["bias"], "bf16")
+    if "silu" in kind:
+        ref["act"] = kw["activation"] = "silu"
+    if "gate" in kind:
+        groups = M // 50 if "groups" in kind else 1  # (50 rows: most tiles have several)
+        ref.update(gate=bf16_randn(r, (groups, N)), residual=bf16_randn(r, (M, N)), groups=groups)
+        kw.update(gate=T(qb, ref["gate"], "bf16"), residual=T(qb, ref["residual"], "bf16"), gate_groups=groups)
+    for out in ("bf16", "f32", "e4m3"):
+        if out == "e4m3" and tile_n == 64:
+            continue
+        want, err = epilogue(y, op.sum_error(mags), **ref, out=out)
+        got = qb.qf.gemm_blocks(*t, out_dtype=out, tile_n=tile_n, split_k=1, b_constant=out == "bf16", **kw)
+        got, scale = got if out == "e4m3" else (got, None)
+        check(values(got), scale.to_numpy() if scale else None, want, err, out, f"{M}x{N}x{K} {tile_n} {kind} {out}")
+
+
+@pytest.mark.parametrize("tile_n,N,K", [(64, 1048, 640), (64, 520, 1152), (128, 2056, 640), (128, 1048, 384), (256, 4104, 384), (256, 2056, 1152)])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_several_tiles_of_a_cta_by_experts(qb, tile_n, N, K, act):
+    """The same over runs of experts: full tiles, tiles of few rows (whose copies are small ones), and tiles without tokens among them."""
+    r = util.rng([38, N, K])
+    E = 5
+    rows = [128, 3, 0, 128, 31, 32, 33, 128, -7, 100, 1, 128, 64, 300, 17, 128, 0, 96, 128, 2, 128, 128, 40, 128, 5, 128, 128, 8, 77, 128, 128, 0, 128, 24, 128, 128, 128, 1, 128, 50]
+    experts = [int(e) for e in r.integers(0, E, len(rows))]
+    experts[4], experts[9], experts[20] = -1, E, 1 << 30  # no such experts
+    M = 128 * len(rows)
+    op = Operands(r, M, N, K, experts=E)
+    A, B, sa, sb = op.tensors(qb)
+    tables = T(qb, np.array(experts, np.int32)), T(qb, np.array(rows, np.int32))
+    live = [slice(128 * i, 128 * i + (max(min(n, 128), 0) if 0 <= e < E else 0)) for i, (e, n) in enumerate(zip(experts, rows))]
+    products = [op.product(at, e) if at.stop > at.start else None for at, e in zip(live, experts)]
+    for out in ("bf16", "f32", "e4m3"):
+        if out == "e4m3" and tile_n == 64:
+            continue
+        carrier = {"bf16": np.uint16, "f32": np.float32, "e4m3": np.uint8}[out]
+        o = T(qb, np.full((M, N), 85, carrier), out)
+        so = T(qb, np.full((blocks(N), M), -5.0, np.float32)) if out == "e4m3" else None
+        before = values(o)[0, 0]
+        qb.qf.gemm_grouped_blocks(A, B, sa, sb, *tables, n_experts=E, activation=act, out=o, scale_out=so, tile_n=tile_n)
+        got, scales = values(o), so.to_numpy() if so else None
+        for i, at in enumerate(live):
+            if products[i] is not None:
+                y, mags = products[i]
+                y, err = epilogue(y, op.sum_error(mags), act=act, out=out)
+                check(got[at], scales[:, at] if so else None, y, err, out, f"tile {i} {tile_n} {out}")
+            assert np.all(got[at.stop : 128 * (i + 1)] == before)  # left as they were
+            if so:
+                assert np.all(scales[:, at.stop : 128 * (i + 1)] == -5.0)
