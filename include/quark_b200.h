@@ -448,7 +448,8 @@ int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scal
  *   experts[m, :] = the top_k experts by c inside them, in order of decreasing c; equal values: the lower group or expert first
  *   weights[m, j] = s of that expert / (the sum of the chosen ones', with renormalize) * factor
  * Choices are made on c as the formula has it, not on a rounding to f32.  A logit of -inf has score 0, and a sum of 0 gives weights
- * 0 (a row without any finite logit).  NaN is chosen last and reaches the weights.  E <= 512, n_groups <= 32, top_k <= 32.
+ * 0 (a row without any finite logit).  A sigmoid of NaN is chosen last, and its weight is NaN (with renormalize all of the token's); a softmax
+ * over NaN or +inf is NaN for the whole row: the token goes to some experts, with NaN for weights.  E <= 512, n_groups <= 32, top_k <= 32.
  * The slot tables (all or none of the five pointers), for n = qb_moe_scored_slots(M, E, top_k) slots, a multiple of 128 that any
  * routing fits: slot_token, slot_weight, tile_expert, token_slot as in qb_moe_route_slots, and tile_rows [n / 128], the slots of each
  * tile that hold a token (0 past the last used tile); with them M <= 2^24.  Workspace (may be NULL without tables and where its size is 0): the first 64 KiB

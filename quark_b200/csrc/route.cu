@@ -348,6 +348,10 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int t, double* scratc
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == none) top = 0.f;
+    bool lost = false;  // NaN or infinity among the logits: the formula's scores are NaN, all of the row's
+#pragma unroll
+    for (int i = 0; i < P; ++i) lost |= !(l[i] < __uint_as_float(0x7f800000u));
+    if (__any_sync(0xffffffffu, lost)) top = __uint_as_float(0x7fffffffu);
     if (kScores || !a.renorm) {
       total = 0.f;
 #pragma unroll

@@ -1129,7 +1129,9 @@ def moe_route_scored(logits, bias=None, *, top_k: int, scoring: str = "softmax",
     ``topk_groups`` of the ``n_groups`` groups of neighbouring experts whose best ``group_top`` values of ``c`` have the largest sum are
     kept, and a token goes to the ``top_k`` experts of largest ``c`` inside them (equal values: the lower group or expert first), with
     the weights ``s`` (over the chosen ones' sum, with ``renormalize``) times ``factor``.  A logit of ``-inf`` scores 0 (a bias of ``-inf``
-    takes an expert out of the choice while others are left); where the chosen scores sum to 0, the weights are 0.  ``out``: the seven tensors of a ``Routing`` to be written (the first two with ``tables=False``)."""
+    takes an expert out of the choice while others are left); where the chosen scores sum to 0, the weights are 0.  A sigmoid of NaN is chosen
+    last; a softmax over NaN or ``+inf`` is NaN for the whole row, and so are the token's weights.  ``out``: the seven tensors of a ``Routing``
+    to be written (the first two with ``tables=False``); with tables at most 2^24 tokens."""
     who = "qf.moe_route_scored"
     if out is not None:
         rc = _fast.route_scored(logits, bias, top_k, scoring, n_groups, topk_groups, group_top, renormalize, factor, tables, out, _WS, _s())

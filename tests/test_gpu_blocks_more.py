@@ -206,3 +206,26 @@ def test_several_tiles_of_a_cta_by_experts(qb, tile_n, N, K, act):
             assert np.all(got[at.stop : 128 * (i + 1)] == before)  # left as they were
             if so:
                 assert np.all(scales[:, at.stop : 128 * (i + 1)] == -5.0)
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("E,groups,kept,top", [(64, 1, 1, 1), (64, 8, 4, 2), (64, 8, 4, 1), (160, 8, 3, 2)])
+def test_a_softmax_over_nan_or_infinity(qb, biased, renorm, E, groups, kept, top):
+    """All of such a row's scores are NaN by the formula, so all of its weights are, whichever experts it goes to; other rows do not see it."""
+    r = util.rng([39, E])
+    x = r.standard_normal((70, E)).astype(np.float32)
+    clean = x.copy()
+    x[10, 5], x[20], x[30, ::2], x[40, E - 1], x[50, 3], x[51, 7] = np.nan, np.nan, np.nan, np.inf, np.inf, -np.inf
+    x[50, 4] = np.nan
+    clean[51, 7] = -np.inf
+    bias = (0.1 * r.standard_normal(E)).astype(np.float32) if biased else None
+    got = qb.qf.moe_route_scored(T(qb, x), T(qb, bias) if biased else None, top_k=4, n_groups=groups, topk_groups=kept, group_top=top, renormalize=renorm)
+    e, w = got.experts.to_numpy(), got.weights.to_numpy()
+    assert e.min() >= 0 and e.max() < E and all(len(set(row)) == 4 for row in e)
+    bad = [10, 20, 30, 40, 50]
+    rest = np.setdiff1d(np.arange(70), bad)
+    assert np.all(np.isnan(w[bad]))
+    we, ww = route(clean, bias, 4, "softmax", groups, kept, top, renorm)
+    np.testing.assert_array_equal(e[rest], we[rest])
+    np.testing.assert_allclose(w[rest], ww[rest], rtol=40 * 2.0**-24)
