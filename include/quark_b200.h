@@ -399,7 +399,7 @@ int32_t qb_patch_scatter(const void* tokens_in, void* latent_out, int32_t C, int
 
 /* ------------------------------------------------------------------ block-scaled e4m3
  * Extensions (the reference's e4m3 has no scales): one f32 scale per 128 values of the contraction, for activations per row
- * (1 x 128 groups), for weights per 128 rows (128 x 128 tiles), the form in which 8-bit checkpoints carry their weights.
+ * (1 x 128 groups), for weights per 128 rows (128 x 128 tiles).
  *
  *   scale = max(max |x| / 448, 2^-126), 1 for a block of zeros; pow2: rounded up to a power of two
  *   q     = e4m3(x * (1 / scale))                the quotient, the reciprocal and the product rounded to nearest in f32
@@ -429,7 +429,7 @@ typedef struct {
   int32_t activation;  /* 0 none, 1 SiLU */
   int32_t gate_groups; /* as qb_gemm_params */
   int32_t pow2;        /* e4m3 C: scales that are powers of two */
-  int32_t b_constant;  /* as bit 1 of qb_gemm_params.reserved; covers b_scale too */
+  int32_t b_constant;  /* as bit 1 of qb_gemm_params.reserved, for B (b_scale is read behind the wait); grouped: no effect */
   int32_t tile_n;      /* 0 = choose; 64, 128 or 256 (an e4m3 C: 128 or 256) */
   int32_t split_k;     /* 0 = choose; 1, 2, 4 or 8 K slices (more than one: tiles of 64 columns, not grouped; one where K has too few blocks) */
 } qb_gemm_blocks_params;
@@ -447,7 +447,7 @@ int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scal
  *   the topk_groups of the n_groups groups of E / n_groups neighbouring experts whose best group_top values of c have the largest sum
  *   experts[m, :] = the top_k experts by c inside them, in order of decreasing c; equal values: the lower group or expert first
  *   weights[m, j] = s of that expert / (the sum of the chosen ones', with renormalize) * factor
- * Choices are made on c as the formula has it, not on a rounding to f32.  A logit of -inf has score 0, and a sum of 0 gives weights
+ * Choices are made on c in 64 bits wherever 32 do not tell (on the logits where c grows with them alone: no bias, and no groups or group_top 1).  A logit of -inf has score 0, and a sum of 0 gives weights
  * 0 (a row without any finite logit).  A sigmoid of NaN is chosen last, and its weight is NaN (with renormalize all of the token's); a softmax
  * over NaN or +inf is NaN for the whole row: the token goes to some experts, with NaN for weights.  E <= 512, n_groups <= 32, top_k <= 32.
  * The slot tables (all or none of the five pointers), for n = qb_moe_scored_slots(M, E, top_k) slots, a multiple of 128 that any

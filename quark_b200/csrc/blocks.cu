@@ -61,7 +61,7 @@ struct Vec8 {
 };
 
 // 1 x 128 groups: 8 lanes to a group, 16 values each, so that the scale is worked out by few lanes and a lane stores 16 bytes.  8192 x 8192
-// bf16: 42.4 us with 16 lanes to a group and four groups to a thread, 33.4 with 8 and two, 32.5 (6.2 TB/s) with one.
+// bf16: 42.4 us with 16 lanes to a group and four groups to a thread, 33.4 with 8 and two, 31.7 - 32.5 (6.3 TB/s) with one; f32 49.2 (6.8 TB/s).
 template <bool F32>
 __global__ void __launch_bounds__(256) quantize_groups_kernel(const void* X, const int* row_index, uint8_t* out, float* scale_out, int units, int kb_total, int rows,
                                                                int src_rows, int cols, int pow2) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) quantize_groups_kernel(const void* X, con
 }
 
 // 128 x 128 tiles: a CTA holds its tile in registers, 16 lanes to a row.  A CTA first reads, then writes, so four of them (two, f32) share an
-// SM: 8192 x 8192 bf16 40.5 -> 34.4 us, and 32.9 (6.1 TB/s) past the caches.
+// SM: 8192 x 8192 bf16 40.5 -> 34.4 us, and 32.9 (6.1 TB/s) past the caches, one launch behind the other; f32 49.8 (6.7 TB/s).
 template <bool F32>
 __global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_tiles_kernel(const void* X, uint8_t* out, float* scale_out, int kb_total, int rb_total, int rows, int cols, int pow2) {
   __shared__ float tops[8];

@@ -1,8 +1,8 @@
 // Matrix products of block-scaled e4m3 operands: C[m, n] = epilogue(sum over blocks b of 128 along K of
 // a_scale[b, m] * b_scale[n / 128, b] * (A[m, block b] . B[n, block b])), dense and grouped by expert.
 //
-// The scales change along the contraction, so the tensor cores can sum one block only: four MMAs (32 of K each) fill one of four TMEM
-// buffers of BN columns, and while they fill the next ones, eight warps read it and add it, scaled, to sums in registers (f32; two
+// The scales are any f32 and change along the contraction, so the tensor cores sum one block only: four MMAs (32 of K each) fill one of four
+// TMEM buffers of BN columns (one of two with 256), and while they fill the next ones, eight warps read it and add it, scaled, to sums in registers (f32; two
 // warps share a TMEM lane quarter, a thread has half a row).  A block of K is one stage of the operand ring: 128 rows x 128 bytes of A,
 // BN x 128 of B.  When the last block is in, the sums go back to TMEM, from where the plain epilogue takes them 16 columns at a time.
 //
@@ -13,11 +13,13 @@
 //   - the warps that sum took 865 with the scales loaded four blocks ahead (a load waits behind the operands, over 1000 clocks), 580 - 690
 //     with 16 warps of half the columns (what every warp does once a block filled the schedulers), and take 330 (64 columns) and 420 (128).
 // 24.5 -> 16.4 us (64) and 28.3 -> 18.6 us (128) at that size.  With all SMs at work the operands' way out of L2 is a bound beside it: a block of 128 columns, 32 KB a
-// CTA, takes 540 clocks then (13.4 TB/s).  256 columns, 840 clocks, need a quarter less of it and few CTAs' rounds: 4096^3 75 us in 128, 78 in 256 (1.8 PFLOP/s),
-// 8192^3 632 us in 256 (1.7 PFLOP/s, at the clock that the power limit leaves).
+// CTA, takes 540 clocks then (13.4 TB/s).  256 columns, 840 clocks, need a quarter less of it and half the epilogues: they win where K is short, 128 where it is
+// long.  8192 x 8192, us in 128 / 256 columns: K = 512 92 - 102 / 80, 1024 115 - 120 / 106 - 111, 2048 180 - 207 / 181 - 212, 4096 324 - 338 / 372 - 409,
+// 8192 603 - 651 / 633 - 699 (1.7 - 1.9 PFLOP/s, at the clock that the power limit leaves); 4096^3 74 / 78 - 93.
 //
 // A CTA stays for all tiles of its share: while its warps are in the epilogue of one, the copies and the MMAs of the next go on (8192^3 814 -> 632 us,
-// 512 x 8192 x 2048 narrowed with SiLU 21.9 -> 17.4 with that, 256 columns and results narrowed from registers).
+// 512 x 8192 x 2048 narrowed with SiLU 21.9 -> 17.4 with that, tiles of 256 columns and results narrowed from registers).  A tile begins with buffer 0 and its epilogue
+// keeps the last block's, so where that is buffer 0 too (4 i + 1 blocks; with 256 columns an odd number) the next tile's first products wait for the epilogue.
 // Warp 0 TMA, warp 1 MMA, warps 2-9 (4-11 with 256 columns) sums and epilogue.  K slices are the CTAs of a cluster, as in gemm.cu (64-column tiles).
 #include <atomic>
 
@@ -581,7 +583,7 @@ static BlockPlan plan_blocks(const qb_gemm_blocks_params& p, int row_tiles) {
       const long tiles = static_cast<long>(row_tiles) * ((p.N + bn - 1) / bn);
       // Measured: ns per block of K (more where the operands of over a hundred CTAs share the way out of L2), what a tile adds, and the
       // set-up of a launch.  Slices add their exchange, which grows with the CTAs that push at once.
-      const long slots = s == 4 ? 33 : s == 8 ? 15 : sms / s;  // clusters that run at once
+      const long slots = s == 4 ? 33 : s == 8 ? 15 : sms / s;  // clusters that run at once (counted on a B200 of 148 SMs; the driver is not asked)
       const long rounds = (tiles + slots - 1) / slots;
       const bool busy = tiles * s > 100;
       const double per_kb = bn == 64 ? 195.0 : bn == 128 ? (busy ? 290.0 : 230.0) : (busy ? 600.0 : 530.0);

@@ -7,7 +7,14 @@
 //
 // A choice compares numbers that may lie next to one another, so it is made on what the formula says and not on a rounding of it:
 // where c grows with l alone (no bias, groups by their best one) on the logits themselves, else on c in 32 bits as long as what it
-// compares lies apart by more than those are off, and in 64 bits for a token where it does not.  Weights are f32.
+// compares lies apart by more than those are off, and in 64 bits for a token where it does not.  Weights are f32, in 64 bits where
+// chosen scores leave it.
+//
+// The choice in 32 bits (select_fast) takes every number of experts without groups, and groups of whole lanes, a power of two of them, at P = 1, 2, 4,
+// 8 or 16 experts to a lane (E / 32 rounded up to one of these).  Others (24 experts in 4 groups, 40, 72, 96, 160, 192, 320 or 384 in 8) go the slow way
+// (select_exact) for every token, and where the choice is on c, all of it in 64 bits.  8192 tokens, 8 groups, sigmoid with a bias, us with tables: 256 experts
+// 20.9, 512 32; 96 25, 160 37, 192 42, 320 76, 384 88 (one token: 256 6.2, 160 10.4, 384 17.6).  So do choices of 32 of more experts on c, since the 33rd has no
+// lane to be compared in, and of 31 where two candidates are close (256 experts without groups and tables: top_k 30 18.7, 31 28.5, 32 59.5).
 //
 // A warp takes a token; its lanes hold P consecutive experts each.  The tables need, for every choice, how many earlier tokens chose
 // the same expert: a block's tokens are a 64-bit mask per expert (rank = set bits below the token), and blocks are joined by the
@@ -16,7 +23,7 @@
 // What bounds it: a token of 256 experts in 8 groups is about 1100 instructions, so 8192 tokens take 13 us of issue slots (6.5 us 2048); among 512 or more
 // there is likely one with a comparison that needs the 64 bits, 1.5 us that nothing hides (3.7 with all of its scores in 64 bits instead of two to a lane:
 // 512 tokens 12.3 us with their tables instead of 9.6, 8192 24.9 instead of 20.9).  The tables add 3.7 - 8 us, a chain of trips to L2.  Every block adds up
-// the counts of all, which past 10,000 tokens grows with their square (65536 tokens: 70 of 170 us).
+// the counts of all, which past 10,000 tokens grows with their square (65536 tokens: 70 of 163 us, 2^18 0.9 of 1.2 ms, 2^20 12 of 14).
 #include <atomic>
 
 #include "common.cuh"

@@ -458,7 +458,8 @@ def gemm_blocks(A, B, a_scale, b_scale, *, out_dtype=None, activation=None, bias
     (``tile_rows=128``); any f32 scales do.
 
     An e4m3 result (``out_dtype="e4m3"``, or an e4m3 ``out``) is narrowed with scales of its own and returned as ``(out, scale_out)``, the A operand
-    of a following product.  ``b_constant`` as in ``gemm``, for ``B`` and ``b_scale``."""
+    of a following product.  ``b_constant`` as in ``gemm``, for ``B`` (``quantize_e4m3_blocks`` lets the calls behind it begin early: a weight
+    that it has just narrowed is constant once the stream has been waited for)."""
     who = "qf.gemm_blocks"
     if out is not None:
         rc = _fast.gemm_blocks(A, B, a_scale, b_scale, out_dtype, activation, bias, gate, residual, gate_groups, out, scale_out, pow2, b_constant, tile_n, split_k, _s())
@@ -497,7 +498,8 @@ def gemm_grouped_blocks(A, B, a_scale, b_scale, tile_expert, tile_rows, *, n_exp
                         b_constant=False, tile_n=0):  # fmt: skip
     """``gemm_blocks`` over 128-row tiles of slot-sorted rows, every tile with the weights of its expert (``gemm_grouped``): ``B`` is
     ``[n_experts * N, K]`` and ``b_scale [n_experts, ceil(N / 128), ceil(K / 128)]`` (``quantize_e4m3_blocks`` of ``[n_experts, N, K]``).
-    The first ``tile_rows[i]`` rows of tile ``i`` are written, the others, and tiles without an expert, are left as they are."""
+    The first ``tile_rows[i]`` rows of tile ``i`` are written, the others, and tiles without an expert, are left as they are.  ``b_constant``
+    is taken as by ``gemm_blocks`` and has no effect: the tables come from a kernel before, so nothing is fetched ahead of it."""
     who = "qf.gemm_grouped_blocks"
     if out is not None:
         rc = _fast.gemm_grouped_blocks(A, B, a_scale, b_scale, tile_expert, tile_rows, n_experts, out_dtype, activation, out, scale_out, pow2, b_constant, tile_n, _s())
