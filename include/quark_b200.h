@@ -420,7 +420,8 @@ int32_t qb_quantize_e4m3_blocks(const void* X, const int32_t* row_index, void* o
 
 /* C[m, n] = epilogue(sum over blocks b of 128 along K of (a_scale[b, m] * b_scale[n / 128, b]) * (A[m, block b] . B[n, block b]))
  * A [M, K], B [N, K] e4m3, a_scale [ceil(K / 128), M], b_scale [ceil(N / 128), ceil(K / 128)] f32; the sums in f32.  Epilogue as
- * qb_gemm: -> + bias[n] -> SiLU -> * gate[m / (M / G), n] + residual[m, n] -> cast.  An e4m3 C is narrowed with scales of its own,
+ * qb_gemm: -> + bias[n] -> SiLU -> * gate[m / (M / G), n] + residual[m, n] -> cast.  SiLU of an f32 or e4m3 result is x / (1 + e^-x) in f32,
+ * 0 below x = -87.3 (less than 1.1e-36 is lost; a group of such results alone is narrowed as zeros).  An e4m3 C is narrowed with scales of its own,
  * c_scale [ceil(N / 128), M] as by qb_quantize_e4m3_blocks from the f32 results: the A operand of a following product.  Else
  * c_scale is NULL.  K a multiple of 16, N of 8; matrices 16-byte aligned.  Needs no workspace. */
 typedef struct {

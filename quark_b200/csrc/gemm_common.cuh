@@ -67,6 +67,7 @@ struct GemmArgs {
 };
 
 // SiLU of a GEMM's epilogue.  kPrecise: where the approximation's 2^-11 would be seen in the result (f32, or e4m3 with scales of its own).
+// (__fdividef by more than 2^126 is 0: below x = -87.3 less than 1.1e-36 is lost.)
 template <bool kPrecise>
 __device__ __forceinline__ float epilogue_silu(float x) {
   return kPrecise ? __fdividef(x, 1.f + __expf(-x)) : silu_fast(x);
