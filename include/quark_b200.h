@@ -451,6 +451,7 @@ int32_t qb_gemm_grouped_blocks(const void* A, const void* B, const float* a_scal
  * Choices are made on c in 64 bits wherever 32 do not tell (on the logits where c grows with them alone: no bias, and no groups or group_top 1).  A logit of -inf has score 0, and a sum of 0 gives weights
  * 0 (a row without any finite logit).  A sigmoid of NaN is chosen last, and its weight is NaN (with renormalize all of the token's); a softmax
  * over NaN or +inf is NaN for the whole row: the token goes to some experts, with NaN for weights.  E <= 512, n_groups <= 32, top_k <= 32.
+ * Fastest without groups to leave out, or with groups of a power of two of experts; others, and top_k 31 and 32, cost up to five times as much.
  * The slot tables (all or none of the five pointers), for n = qb_moe_scored_slots(M, E, top_k) slots, a multiple of 128 that any
  * routing fits: slot_token, slot_weight, tile_expert, token_slot as in qb_moe_route_slots, and tile_rows [n / 128], the slots of each
  * tile that hold a token (0 past the last used tile); with them M <= 2^24.  Workspace (may be NULL without tables and where its size is 0): the first 64 KiB

@@ -7,7 +7,7 @@ import pytest
 from oracle import codec
 from tests import util
 from tests.test_gpu_blocks import Operands, T, blocks, check, check_routing, epilogue, route, route_scores, values
-from tests.util import bf16_randn
+from tests.util import bf16_randn, f32
 
 pytestmark = pytest.mark.gpu
 
@@ -69,6 +69,48 @@ def test_parameters_loaded_into_a_model_that_was_prepared(qb, kw):
     np.testing.assert_array_equal(got[0], want[1])
     np.testing.assert_array_equal(got[1], want[0])
     assert np.any(want[0] != want[1])
+
+
+@pytest.mark.parametrize("first", ["bf16", "e4m3", "blocks"])
+@pytest.mark.parametrize("second", ["bf16", "e4m3", "blocks"])
+@pytest.mark.parametrize("fuse", [False, True])
+def test_an_mlp_of_linears_narrowed_each_as_it_likes(qb, first, second, fuse):
+    from quark_b200 import nn
+
+    forms = {"bf16": {}, "e4m3": dict(fp8=True), "blocks": dict(fp8=True, fp8_blocks=True)}
+    r = util.rng(40)
+    M, D, H = 33, 256, 640
+    w1, w2, x = bf16_randn(r, (H, D), 0.06), bf16_randn(r, (D, H), 0.04), bf16_randn(r, (M, D))
+    mlp = nn.MLP(D, H, D, fuse_silu=fuse)
+    mlp.fc1.load_weight(T(qb, w1, "bf16"))
+    mlp.fc2.load_weight(T(qb, w2, "bf16"))
+    mlp.fc1.prepare(**forms[first])
+    mlp.fc2.prepare(**forms[second])
+    got = f32(mlp(T(qb, x, "bf16")).to_numpy(), "bf16")
+    f = lambda t: f32(t, "bf16").astype(np.float64)  # noqa: E731
+    h = f(x) @ f(w1).T
+    want = (h / (1 + np.exp(-h))) @ f(w2).T
+    # four operands, each off by at most 2^-4 of itself (without scales 2^-10 absolute as well: of weights of 0.04 another 2^-5), or 2^-8
+    step = {"bf16": 2.0**-8, "blocks": 2.0**-4, "e4m3": 2.0**-4 + 2.0**-5}
+    assert np.linalg.norm(got - want) <= 2 * (step[first] + step[second] + 2.0**-8) * np.linalg.norm(want)
+
+
+def test_a_state_with_its_scales_goes_from_layer_to_layer(qb):
+    """As tensors and as host arrays: the layer that takes it gives what the other gave."""
+    from quark_b200 import nn
+
+    r = util.rng(41)
+    x = T(qb, bf16_randn(r, (9, 384)), "bf16")
+    lins = [nn.Linear(384, 200) for _ in range(3)]
+    for lin in lins:
+        lin.load_weight(T(qb, bf16_randn(r, (200, 384), 0.05), "bf16"))
+        lin.prepare(fp8=True, fp8_blocks=True)
+    want = lins[0](x).to_numpy()
+    assert np.any(lins[1](x).to_numpy() != want)
+    lins[1].load_state_dict(lins[0].state_dict())
+    lins[2].load_state_dict({k: v.to_numpy() for k, v in lins[0].state_dict().items()})
+    for lin in lins[1:]:
+        np.testing.assert_array_equal(lin(x).to_numpy(), want)
 
 
 # -------------------------------------------------------------------------------------------------------------- routing
