@@ -306,7 +306,7 @@ class Engine:
                 noise = self._rng.standard_normal(n, dtype=np.float32)
             self._noise_host.array[:] = self._to_bf16(noise)
             self._h2d(self._noise_dev, self._noise_host.ptr, n * 2)
-        if self._use_graph and self.gen._graph is None:
+        if self._use_graph and not self.gen.captured():
             self._capture()
         if self._watchdog is not None:  # the guard ends only when the frame has: the host waits for the stream inside it
             with self._watchdog.guard():

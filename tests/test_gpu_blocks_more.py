@@ -71,6 +71,31 @@ def test_parameters_loaded_into_a_model_that_was_prepared(qb, kw):
     assert np.any(want[0] != want[1])
 
 
+@pytest.mark.parametrize("kw", [dict(fp8_blocks=True), dict(fp8_blocks=False), dict(fp8_blocks=True, moe=True, moe_n_experts=8, moe_top_k=2)])
+def test_parameters_loaded_into_a_session_that_replays_its_frames(qb, kw):
+    """Frames are captured before the other parameters come, and again behind them: a frame is the one of a session that calls one by one."""
+    from quark_b200.models import QuantConfig, Waypoint15Config, make_params
+    from tests.test_gpu_model import small_cfg
+
+    quant = QuantConfig(linear="fp8", kv_cache="bf16", attn_compute="bf16", moe="fp8")
+    cfg = Waypoint15Config(**{**small_cfg(qb, "bf16").__dict__, "quant": quant, **kw})
+    params = [make_params(cfg, seed=s, weight_std=0.04) for s in (42, 43)]
+    r = util.rng(44)
+    noise = [r.standard_normal((1, cfg.latent_numel)).astype(np.float32) for _ in range(5)]
+    frames = []
+    for graph in (True, False):
+        eng = qb.Engine(cfg=cfg, quant=quant, params=params[0], use_graph=graph)
+        out = [eng.gen_frame(noise=n) for n in noise[:2]]
+        eng.model.load_params(params[1])
+        eng.model.prepare()
+        out += [eng.gen_frame(noise=n) for n in noise[2:4]]
+        assert (eng.gen._graph is not None) == graph
+        eng.model.load_state_dict({k: v.to_numpy().copy() for k, v in eng.model.state_dict().items()})  # the same values in other memory
+        frames.append(out + [eng.gen_frame(noise=noise[4])])
+    for a, b in zip(*frames):
+        np.testing.assert_array_equal(a, b)
+
+
 @pytest.mark.parametrize("first", ["bf16", "e4m3", "blocks"])
 @pytest.mark.parametrize("second", ["bf16", "e4m3", "blocks"])
 @pytest.mark.parametrize("fuse", [False, True])
