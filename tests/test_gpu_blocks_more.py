@@ -96,6 +96,39 @@ def test_parameters_loaded_into_a_session_that_replays_its_frames(qb, kw):
         np.testing.assert_array_equal(a, b)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(), dict(fp8_scales=True), dict(ctrl_conditioning=True), dict(value_residual=False), dict(quilt_factor=2),
+    dict(moe=True, moe_n_experts=32, moe_top_k=4, moe_scoring="softmax", moe_n_groups=8, moe_topk_groups=3, moe_renormalize=False),
+])  # fmt: skip
+def test_sessions_with_everything_in_e4m3(qb, kw):
+    """Block-scaled linears beside e4m3 caches and attention (the default of ``Engine``): the wirings that a block can have give the same
+    bits, replayed or not, and stay close to the session without block scales and to the one in bf16."""
+    from quark_b200.models import QuantConfig, Waypoint15Config, make_params
+    from tests.test_gpu_model import small_cfg
+
+    quant = QuantConfig.all_fp8()
+    cfg = Waypoint15Config(**{**small_cfg(qb, "bf16").__dict__, "quant": quant, "fp8_blocks": True, **kw})
+    params = make_params(cfg, seed=45, weight_std=0.04)
+    r = util.rng(46)
+    lats = [codec.f32_to_bf16(r.standard_normal((1, cfg.latent_numel)).astype(np.float32)) for _ in range(3)]
+    noise = r.standard_normal((1, cfg.latent_numel)).astype(np.float32)
+    ctrl = qb.CtrlInput(button={1, 5}, mouse=(0.3, -0.2)) if cfg.ctrl_conditioning else None
+    outs = []
+    wide = dict(quant=QuantConfig.all_bf16(), fp8_blocks=False, fp8_scales=False)
+    for graph, other in ((True, {}), (False, {}), (False, dict(fuse_qkv_post=False)), (False, dict(fp8_blocks=False)), (False, wide)):
+        c = Waypoint15Config(**{**cfg.__dict__, **other})
+        eng = qb.Engine(cfg=c, quant=c.quant, params=params, use_graph=graph)
+        for lat in lats:
+            eng.append_frame(lat, ctrl) if ctrl else eng.append_frame(lat)
+        outs.append([(eng.gen_frame(ctrl, noise=noise) if ctrl else eng.gen_frame(noise=noise)).reshape(-1) for _ in range(2)])
+    for o in outs[1:3]:
+        for a, b in zip(outs[0], o):
+            np.testing.assert_array_equal(a, b)
+    # as in test_sessions of the layers' file: linears off by 2 - 3 % (rms) each; caches and probabilities in e4m3 add as much again
+    assert util.cosine(f32(outs[0][0], "bf16"), f32(outs[4][0], "bf16")) >= 0.95
+    assert np.any(outs[0][0] != outs[3][0])
+
+
 @pytest.mark.parametrize("first", ["bf16", "e4m3", "blocks"])
 @pytest.mark.parametrize("second", ["bf16", "e4m3", "blocks"])
 @pytest.mark.parametrize("fuse", [False, True])
